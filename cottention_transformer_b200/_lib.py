@@ -55,12 +55,18 @@ _SIGNATURES = {
     "cott_rotary": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_longlong, _I, _I, _P],
     "cott_cos_attn_fwd_rotary": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "cott_cos_attn_bwd_rotary": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "cott_gated_scan_fwd": [_P] * 11 + [_I] * 6 + [_P],
+    "cott_gated_scan_bwd": [_P] * 5 + [_I] + [_P] * 10 + [_I] * 6 + [_P],
+    "cott_gated_step": [_P] * 7 + [_I] * 6 + [_P],
+    "cott_qk_norm_fwd": [_P] * 8 + [_I] * 5 + [ctypes.c_float, _I, _I, _P],
+    "cott_qk_norm_bwd": [_P] * 13 + [_I] * 5 + [ctypes.c_float, _I, _I, _P],
     "cott_check_status": [ctypes.POINTER(ctypes.c_int)],
     "cott_selftest_device_wait": [_I, _I, _I, _P],
 }
 _STR = {"cott_version": [], "cott_last_error": [], "cott_status_string": [_I]}
 _SIZE = {"cott_bidir_scratch_bytes": [_I, _I, _I, _I, _I, _I], "cott_cos_attn_saved_bytes": [_I, _I, _I],
-         "cott_cos_attn_wide_workspace_bytes": [_I, _I, _I], "cott_cos_attn_f32_workspace_bytes": [_I, _I, _I, _I], "cott_cos_attn_seg_workspace_bytes": [_I, _I, _I, _I]}
+         "cott_cos_attn_wide_workspace_bytes": [_I, _I, _I], "cott_cos_attn_f32_workspace_bytes": [_I, _I, _I, _I], "cott_cos_attn_seg_workspace_bytes": [_I, _I, _I, _I],
+         "cott_gated_scan_states_bytes": [_I] * 5, "cott_gated_scan_workspace_bytes": [_I] * 6, "cott_qk_norm_workspace_bytes": [_I] * 5}
 
 class CottRotaryTables(ctypes.Structure):
     """``cott_rotary_tables``: fp32 sin / cos tables, the rotary dim and the element stride between batch entries."""
@@ -71,6 +77,21 @@ class CottRotaryTables(ctypes.Structure):
 class CottLayout(ctypes.Structure):
     """``cott_layout``: element strides (batch, head, position) of q/k/v/dq/dk/dv and of out/dout."""
     _fields_ = [(n, ctypes.c_longlong) for n in ("in_b", "in_h", "in_n", "out_b", "out_h", "out_n")]
+
+
+class CottStrides(ctypes.Structure):
+    """``cott_strides``: elements between two batch entries, heads, positions."""
+    _fields_ = [(n, ctypes.c_longlong) for n in ("b", "h", "n")]
+
+
+class CottGatedLayout(ctypes.Structure):
+    """``cott_gated_layout``: where the tensors of the gated scan lie."""
+    _fields_ = [(n, CottStrides) for n in ("q", "k", "v", "out", "gate", "dq", "dk", "dv", "dgate")]
+
+
+class CottNormLayout(ctypes.Structure):
+    """``cott_norm_layout``: where the tensors of the q/k norm lie."""
+    _fields_ = [(n, CottStrides) for n in ("q", "k", "q_out", "k_out", "dq", "dk")]
 
 
 _lib = None

@@ -1,0 +1,325 @@
+// RMS norm of every head of q and k with a learned weight, and the rotary embedding ("rotate every two"), in one pass:
+//     n = x rsqrt(mean x^2 + eps)      y = Rot(n w)
+// and its backward, with e = Rot^T dy, f = e w:
+//     dw = sum over all rows of e n            dx = r (f - n mean(f n)),  r = rsqrt(mean x^2 + eps)
+// A row (one head of one position) is spread over D/8 lanes (16 bits) or D/4 lanes (fp32) that own one 16-byte piece each, so every
+// access is a whole 16 bytes, pairs of the rotation stay inside a lane and the row sums are shuffles.  fp32 arithmetic, one rounding.
+// HBM-bound: every input is read once and every output written once; the backward recomputes r from x.  The gradient of a weight is
+// summed in registers over the rows of a thread, over the CTA in shared memory and over the CTAs by a second small kernel, all in a
+// fixed order.
+#include "common.cuh"
+
+using namespace cott;
+
+namespace {
+
+constexpr int kNormThreads = 256;
+
+template <typename T> struct Piece {
+  static constexpr int kElems = 16 / sizeof(T);
+  union {
+    uint4 u;
+    T e[kElems];
+  };
+  __device__ __forceinline__ Piece() {}
+};
+
+struct NormSide {  // q or k
+  const void *x, *w, *dy;
+  void *y, *dx;
+  cott_strides sx, sy, sdy, sdx;
+  int H;
+  unsigned rows;  // B * N * H
+};
+struct NormArgs {
+  NormSide side[2];
+  const float *sin_t, *cos_t;
+  float* partial;  // backward: [2][CTAs][D]
+  long long table_batch_stride;
+  int N, rot, w_f32;
+  float eps;
+};
+
+// The row numbered `r` of a side: consecutive numbers walk the heads of a position, then the positions, then the batch.
+struct RowAt {
+  int b, n, h;
+};
+__device__ __forceinline__ RowAt row_at(unsigned r, int H, int N) {
+  const unsigned p = r / static_cast<unsigned>(H), b = p / static_cast<unsigned>(N);
+  return RowAt{static_cast<int>(b), static_cast<int>(p - b * N), static_cast<int>(r - p * H)};
+}
+__device__ __forceinline__ long long at(const cott_strides& s, const RowAt& r) { return r.b * s.b + r.h * s.h + r.n * s.n; }
+
+template <int LPR>
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+  for (int off = LPR / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+// the lane's E weights
+template <typename T, int E>
+__device__ __forceinline__ void load_weights(float (&w)[E], const void* src, int f32, int c) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) w[e] = f32 ? static_cast<const float*>(src)[c + e] : to_acc(static_cast<const T*>(src)[c + e]);
+}
+// rotates the lane's E/2 pairs; `sign` = -1: the transposed rotation
+template <int E>
+__device__ __forceinline__ void rotate(float (&x)[E], const float* sin_t, const float* cos_t, float sign) {
+  float s[E / 2], c[E / 2];
+  if constexpr (E == 8) {
+    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_t);
+    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cos_t);
+  } else {
+    *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(sin_t);
+    *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cos_t);
+  }
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    float xo, yo;
+    rot_pair(x[2 * i], x[2 * i + 1], c[i], sign * s[i], xo, yo);
+    x[2 * i] = xo, x[2 * i + 1] = yo;
+  }
+}
+
+// grid = (CTAs, 2): y = q, k.  Each CTA takes every gridDim.x-th group of rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_fwd_kernel(const NormArgs a) {
+  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;  // elements and lanes of a piece, rows per CTA and round
+  const NormSide& s = a.side[blockIdx.y];
+  const int piece = threadIdx.x % LPR, c = piece * E;
+  pdl_allow_next();
+  pdl_wait_prior();
+  float w[E];
+  load_weights<T, E>(w, s.w, a.w_f32, c);
+  for (unsigned r0 = blockIdx.x * RPC; r0 < s.rows; r0 += gridDim.x * RPC) {
+    const unsigned r = r0 + threadIdx.x / LPR;
+    const bool in = r < s.rows;
+    const RowAt row = row_at(in ? r : s.rows - 1, s.H, a.N);
+    Piece<T> p;
+    p.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row) + c);
+    float x[E], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] = to_acc(p.e[e]);
+      sum = fmaf(x[e], x[e], sum);
+    }
+    const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * rms * w[e];
+    if (c < a.rot) {
+      const long long t = row.b * a.table_batch_stride + static_cast<long long>(row.n) * (a.rot / 2) + c / 2;
+      rotate<E>(x, a.sin_t + t, a.cos_t + t, 1.f);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.e[e] = from_acc<T>(x[e]);
+    if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row) + c) = p.u;
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArgs a) {
+  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;
+  const NormSide& s = a.side[blockIdx.y];
+  const int piece = threadIdx.x % LPR, c = piece * E;
+  __shared__ float part[RPC][D];
+  pdl_allow_next();
+  pdl_wait_prior();
+  float w[E], dw[E];
+  load_weights<T, E>(w, s.w, a.w_f32, c);
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = 0.f;
+  for (unsigned r0 = blockIdx.x * RPC; r0 < s.rows; r0 += gridDim.x * RPC) {
+    const unsigned r = r0 + threadIdx.x / LPR;
+    const bool in = r < s.rows;
+    const RowAt row = row_at(in ? r : s.rows - 1, s.H, a.N);
+    Piece<T> p, d;
+    p.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row) + c);
+    d.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.dy) + at(s.sdy, row) + c);
+    float x[E], f[E], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] = to_acc(p.e[e]);
+      f[e] = to_acc(d.e[e]);
+      sum = fmaf(x[e], x[e], sum);
+    }
+    if (c < a.rot) {
+      const long long t = row.b * a.table_batch_stride + static_cast<long long>(row.n) * (a.rot / 2) + c / 2;
+      rotate<E>(f, a.sin_t + t, a.cos_t + t, -1.f);
+    }
+    const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
+    float dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] *= rms;
+      if (in) dw[e] = fmaf(f[e], x[e], dw[e]);
+      f[e] *= w[e];
+      dot = fmaf(f[e], x[e], dot);
+    }
+    dot = row_sum<LPR>(dot) * (1.f / D);
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.e[e] = from_acc<T>(rms * (f[e] - x[e] * dot));
+    if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row) + c) = p.u;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) part[threadIdx.x / LPR][c + e] = dw[e];
+  __syncthreads();
+  for (int e = threadIdx.x; e < D; e += kNormThreads) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < RPC; ++i) sum += part[i][e];
+    a.partial[(static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * D + e] = sum;
+  }
+}
+
+// dw of q and of k: the sums of the CTAs, in their order.  grid = (D / 32, 2), block = 256: 32 columns, eight threads each.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) qk_norm_dw_kernel(const float* __restrict__ partial, void* dqw, void* dkw, int ctas, int D, int w_f32) {
+  __shared__ float part[8][32];
+  const int col = threadIdx.x & 31, u = threadIdx.x >> 5, e = blockIdx.x * 32 + col;
+  pdl_allow_next();
+  pdl_wait_prior();
+  const float* src = partial + static_cast<long>(blockIdx.y) * ctas * D;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = u; i < ctas; i += 8) sum += src[static_cast<long>(i) * D + e];
+  part[u][col] = sum;
+  __syncthreads();
+  if (u == 0) {
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i][col];
+    void* dst = blockIdx.y ? dkw : dqw;
+    if (w_f32)
+      static_cast<float*>(dst)[e] = sum;
+    else
+      static_cast<T*>(dst)[e] = from_acc<T>(sum);
+  }
+}
+
+int check_norm_args(int B, int Hq, int Hk, int N, int D, int dtype, int weight_dtype, const cott_rotary_tables* rotary) {
+  if (dtype != COTT_F32 && dtype != COTT_F16 && dtype != COTT_BF16)
+    return fail(COTT_ERR_DTYPE, "cott_qk_norm takes float32, float16 or bfloat16 (dtype code %d)", dtype);
+  if (weight_dtype != COTT_F32 && weight_dtype != dtype)
+    return fail(COTT_ERR_DTYPE, "cott_qk_norm: the weights are float32 or of the tensors' type (dtype code %d)", weight_dtype);
+  if (B < 0 || Hq < 0 || Hk < 0 || N < 0) return fail(COTT_ERR_SHAPE, "negative size B=%d Hq=%d Hk=%d N=%d", B, Hq, Hk, N);
+  if (D != 32 && D != 64 && D != 128) return fail(COTT_ERR_SHAPE, "cott_qk_norm supports head dims 32, 64 and 128 (got %d)", D);
+  if ((double)B * N * (Hq > Hk ? Hq : Hk) > 2147483647.0) return fail(COTT_ERR_SHAPE, "B*H*N too large");
+  if (rotary) {
+    if (rotary->rot_dim < 8 || rotary->rot_dim % 8 || rotary->rot_dim > D)
+      return fail(COTT_ERR_SHAPE, "the rotary dim must be a multiple of 8 and at most the head dim (got %d, %d)", rotary->rot_dim, D);
+    if (!rotary->sin_table || !rotary->cos_table) return fail(COTT_ERR_NULL, "null pointer: rotary table");
+    if ((reinterpret_cast<uintptr_t>(rotary->sin_table) | reinterpret_cast<uintptr_t>(rotary->cos_table)) & 15 || rotary->table_batch_stride % 4)
+      return fail(COTT_ERR_ALIGN, "rotary tables must be 16-byte aligned");
+  }
+  return COTT_OK;
+}
+int check_norm_rows(const char* name, const void* p, const cott_strides& s, int dtype) {
+  const long long unit = 16 / (long long)dtype_size(dtype);
+  if (!p) return fail(COTT_ERR_NULL, "null pointer: %s", name);
+  if (reinterpret_cast<uintptr_t>(p) & 15) return fail(COTT_ERR_ALIGN, "%s must be 16-byte aligned", name);
+  if (s.b % unit || s.h % unit || s.n % unit) return fail(COTT_ERR_ALIGN, "the strides of %s must be multiples of 16 bytes", name);
+  return COTT_OK;
+}
+
+int norm_ctas(unsigned rows, int rows_per_cta, int resident) {
+  int sm = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, dev);
+  const long want = ((long)rows + rows_per_cta - 1) / rows_per_cta, most = (long)sm * resident;
+  return (int)(want < 1 ? 1 : want < most ? want : most);
+}
+constexpr int kBwdResident = 3;
+
+template <typename T, int D>
+int launch_norm(const NormArgs& a, bool bwd, void* dqw, void* dkw, cudaStream_t stream) {
+  constexpr int RPC = kNormThreads / (D / Piece<T>::kElems);
+  const unsigned rows = a.side[0].rows > a.side[1].rows ? a.side[0].rows : a.side[1].rows;
+  if (!bwd) {
+    COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D>, dim3(norm_ctas(rows, RPC, 64), 2), kNormThreads, 0, stream, a));
+    return COTT_OK;
+  }
+  const int ctas = norm_ctas(rows, RPC, kBwdResident);
+  COTT_CUDA_TRY(launch_pdl(qk_norm_bwd_kernel<T, D>, dim3(ctas, 2), kNormThreads, 0, stream, a));
+  COTT_CUDA_TRY(launch_pdl(qk_norm_dw_kernel<T>, dim3(D / 32, 2), kNormThreads, 0, stream, static_cast<const float*>(a.partial), dqw, dkw, ctas, D, a.w_f32));
+  return COTT_OK;
+}
+template <typename T>
+int launch_norm_dim(const NormArgs& a, int D, bool bwd, void* dqw, void* dkw, cudaStream_t stream) {
+  switch (D) {
+    case 32: return launch_norm<T, 32>(a, bwd, dqw, dkw, stream);
+    case 64: return launch_norm<T, 64>(a, bwd, dqw, dkw, stream);
+    default: return launch_norm<T, 128>(a, bwd, dqw, dkw, stream);
+  }
+}
+int launch_norm_any(const NormArgs& a, int D, int dtype, bool bwd, void* dqw, void* dkw, cudaStream_t stream) {
+  switch (dtype) {
+    case COTT_F32: return launch_norm_dim<float>(a, D, bwd, dqw, dkw, stream);
+    case COTT_F16: return launch_norm_dim<__half>(a, D, bwd, dqw, dkw, stream);
+    default: return launch_norm_dim<__nv_bfloat16>(a, D, bwd, dqw, dkw, stream);
+  }
+}
+NormArgs norm_args(const cott_norm_layout* l, const void* q, const void* k, const void* qw, const void* kw, const cott_rotary_tables* rotary, int B,
+                   int Hq, int Hk, int N, int D, int weight_dtype, float eps) {
+  NormArgs a = {};
+  const cott_strides dq = {(long long)Hq * N * D, (long long)N * D, D}, dk = {(long long)Hk * N * D, (long long)N * D, D};
+  a.side[0].x = q, a.side[0].w = qw, a.side[0].H = Hq, a.side[0].rows = (unsigned)((long)B * N * Hq), a.side[0].sx = l ? l->q : dq;
+  a.side[1].x = k, a.side[1].w = kw, a.side[1].H = Hk, a.side[1].rows = (unsigned)((long)B * N * Hk), a.side[1].sx = l ? l->k : dk;
+  a.side[0].sy = a.side[0].sdy = l ? l->q_out : dq, a.side[1].sy = a.side[1].sdy = l ? l->k_out : dk;
+  a.side[0].sdx = l ? l->dq : dq, a.side[1].sdx = l ? l->dk : dk;
+  a.N = N, a.w_f32 = weight_dtype == COTT_F32, a.eps = eps;
+  if (rotary) a.sin_t = rotary->sin_table, a.cos_t = rotary->cos_table, a.rot = rotary->rot_dim, a.table_batch_stride = rotary->table_batch_stride;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cott_qk_norm_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const cott_rotary_tables* rotary, void* q_out, void* k_out,
+                     const cott_norm_layout* layout, int B, int Hq, int Hk, int N, int D, float eps, int dtype, int weight_dtype, void* stream) {
+  int st = check_norm_args(B, Hq, Hk, N, D, dtype, weight_dtype, rotary);
+  if (st) return st;
+  if ((long)B * N * (Hq + Hk) == 0) return COTT_OK;
+  NormArgs a = norm_args(layout, q, k, q_weight, k_weight, rotary, B, Hq, Hk, N, D, weight_dtype, eps);
+  a.side[0].y = q_out, a.side[1].y = k_out;
+  if (Hq && ((st = check_norm_rows("q", q, a.side[0].sx, dtype)) || (st = check_norm_rows("q_out", q_out, a.side[0].sy, dtype)))) return st;
+  if (Hk && ((st = check_norm_rows("k", k, a.side[1].sx, dtype)) || (st = check_norm_rows("k_out", k_out, a.side[1].sy, dtype)))) return st;
+  if ((Hq && !q_weight) || (Hk && !k_weight)) return fail(COTT_ERR_NULL, "null pointer: weight");
+  if (!Hq || !Hk) return fail(COTT_ERR_SHAPE, "q and k need a head each");
+  DeviceScope scope(q);
+  COTT_CUDA_TRY(scope.status());
+  return launch_norm_any(a, D, dtype, false, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+size_t cott_qk_norm_workspace_bytes(int B, int Hq, int Hk, int N, int D) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || N <= 0 || D <= 0) return 0;
+  return (size_t)2 * norm_ctas(0x7fffffff, 1, kBwdResident) * D * sizeof(float);
+}
+
+int cott_qk_norm_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const cott_rotary_tables* rotary, const void* dq_out,
+                     const void* dk_out, void* workspace, void* dq, void* dk, void* dq_weight, void* dk_weight, const cott_norm_layout* layout, int B,
+                     int Hq, int Hk, int N, int D, float eps, int dtype, int weight_dtype, void* stream) {
+  int st = check_norm_args(B, Hq, Hk, N, D, dtype, weight_dtype, rotary);
+  if (st) return st;
+  if (!dq_weight || !dk_weight) return fail(COTT_ERR_NULL, "null pointer: weight gradient");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if ((long)B * N * (Hq + Hk) == 0) {
+    DeviceScope scope(dq_weight);
+    COTT_CUDA_TRY(scope.status());
+    COTT_CUDA_TRY(cudaMemsetAsync(dq_weight, 0, D * dtype_size(weight_dtype), s));
+    COTT_CUDA_TRY(cudaMemsetAsync(dk_weight, 0, D * dtype_size(weight_dtype), s));
+    return COTT_OK;
+  }
+  if (!Hq || !Hk) return fail(COTT_ERR_SHAPE, "q and k need a head each");
+  NormArgs a = norm_args(layout, q, k, q_weight, k_weight, rotary, B, Hq, Hk, N, D, weight_dtype, eps);
+  a.side[0].dy = dq_out, a.side[1].dy = dk_out, a.side[0].dx = dq, a.side[1].dx = dk, a.partial = static_cast<float*>(workspace);
+  if ((st = check_norm_rows("q", q, a.side[0].sx, dtype)) || (st = check_norm_rows("k", k, a.side[1].sx, dtype)) ||
+      (st = check_norm_rows("dq_out", dq_out, a.side[0].sdy, dtype)) || (st = check_norm_rows("dk_out", dk_out, a.side[1].sdy, dtype)) ||
+      (st = check_norm_rows("dq", dq, a.side[0].sdx, dtype)) || (st = check_norm_rows("dk", dk, a.side[1].sdx, dtype)))
+    return st;
+  if (!q_weight || !k_weight || !workspace) return fail(COTT_ERR_NULL, "null pointer: %s", workspace ? "weight" : "workspace");
+  DeviceScope scope(q);
+  COTT_CUDA_TRY(scope.status());
+  return launch_norm_any(a, D, dtype, true, dq_weight, dk_weight, s);
+}
+
+}  // extern "C"

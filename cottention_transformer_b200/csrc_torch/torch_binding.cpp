@@ -529,6 +529,221 @@ struct F32Fn : torch::autograd::Function<F32Fn> {
   }
 };
 
+// ---- 4. gated scan, its step, q/k norm with rotation ---------------------------------------------------------------
+// `t` as the kernels read it: rows contiguous, base and strides in multiples of 16 bytes; else a dense copy
+bool rows_fit(const at::Tensor& t) {
+  const int64_t unit = 16 / t.element_size(), d = t.dim() - 1;
+  if (t.stride(d) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t i = 0; i < d; ++i)
+    if (t.size(i) != 1 && (t.stride(i) <= 0 || t.stride(i) % unit)) return false;
+  return true;
+}
+at::Tensor rows16(const at::Tensor& t) { return rows_fit(t) ? t : dense16(t); }
+cott_strides strides3(const at::Tensor& t) {
+  auto s = [&](int i) { return t.size(i) == 1 ? 0LL : (long long)t.stride(i); };
+  return cott_strides{s(0), s(1), s(2)};
+}
+void check_gated(const char* what, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda() && log_decay.is_cuda(), what, " needs CUDA tensors (there is no CPU path)");
+  check_bhnd(q, k, v);
+  const at::ScalarType t = q.scalar_type();
+  TORCH_CHECK((t == at::kFloat || t == at::kHalf || t == at::kBFloat16) && k.scalar_type() == t && v.scalar_type() == t, what,
+              " takes float32, float16 or bfloat16 tensors of one type, got ", t, ", ", k.scalar_type(), " and ", v.scalar_type());
+  const int64_t D = q.size(3);
+  TORCH_CHECK(D == 32 || D == 64 || D == 128, what, " supports head dims 32, 64 and 128 (got ", D, ")");
+  TORCH_CHECK(log_decay.sizes() == q.sizes().slice(0, 3) && (log_decay.scalar_type() == at::kFloat || log_decay.scalar_type() == t),
+              "log_decay must be [B, H, N] = ", q.sizes().slice(0, 3), " in float32 or the tensors' type, got ", log_decay.sizes(), " in ", log_decay.scalar_type());
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device() && log_decay.device() == q.device(), "q, k, v and log_decay must be on one device");
+}
+void check_gated_state(const char* name, const at::Tensor& s, const at::Tensor& q) {
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(3);
+  TORCH_CHECK(s.scalar_type() == at::kFloat && s.sizes() == at::IntArrayRef({B, H, D, D}) && s.device() == q.device(), name,
+              " must be a float32 [B, H, D, D] = ", at::IntArrayRef({B, H, D, D}), " tensor on the tensors' device");
+}
+OptTensor gated_keep(const OptTensor& keep, const at::Tensor& q) {
+  if (!has(keep)) return c10::nullopt;
+  TORCH_CHECK((keep->scalar_type() == at::kBool || keep->scalar_type() == at::kByte) && keep->sizes() == at::IntArrayRef({q.size(0), q.size(2)}) &&
+                  keep->device() == q.device(),
+              "keep must be a bool [B, N] = ", at::IntArrayRef({q.size(0), q.size(2)}), " tensor on the tensors' device");
+  return keep_u8(keep, q);
+}
+float* f32_or_null(const OptTensor& t) { return has(t) ? t->data_ptr<float>() : nullptr; }
+at::Tensor state_like(const at::Tensor& q) { return at::empty({q.size(0), q.size(1), q.size(3), q.size(3)}, q.options().dtype(at::kFloat)); }
+
+using Grads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+Grads gated_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& gate, const OptTensor& keep, bool with_initial,
+                const at::Tensor& states, const at::Tensor& dout_, const OptTensor& dfinal_, bool want_dinitial) {
+  const int B = (int)q.size(0), H = (int)q.size(1), N = (int)q.size(2), D = (int)q.size(3);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor dout = rows16(dout_.scalar_type() == q.scalar_type() ? dout_ : dout_.to(q.scalar_type()));
+  const OptTensor dfinal = has(dfinal_) ? OptTensor(dense16(*dfinal_)) : OptTensor();
+  at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dg = at::empty_like(gate),
+             dinit = want_dinitial ? state_like(q) : at::empty({0}, gate.options().dtype(at::kFloat));
+  const int code = dtype_code(q.scalar_type());
+  const at::Tensor ws = bytes_like(q, cott_gated_scan_workspace_bytes(B, H, N, D, code, 1));
+  const cott_gated_layout lay = {strides3(q),  strides3(k),  strides3(v),  strides3(dout), strides3(gate),
+                                 strides3(dq), strides3(dk), strides3(dv), strides3(dg)};
+  check(cott_gated_scan_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), gate.data_ptr(), u8(keep), with_initial ? 1 : 0, states.data_ptr(),
+                            dout.data_ptr(), f32_or_null(dfinal), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+                            want_dinitial ? dinit.data_ptr<float>() : nullptr, &lay, B, H, N, D, code, dtype_code(gate.scalar_type()), stream_of(q)),
+        "cott_gated_scan_bwd");
+  return {dq, dk, dv, dg, dinit};
+}
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& gate,
+                               const OptTensor& keep, const OptTensor& initial, bool return_state, bool want_dinitial) {
+    const at::Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
+    const OptTensor init = has(initial) ? OptTensor(dense16(*initial)) : OptTensor(), kp = gated_keep(keep, q);
+    const int B = (int)q.size(0), H = (int)q.size(1), N = (int)q.size(2), D = (int)q.size(3), code = dtype_code(q.scalar_type());
+    const c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = at::empty_like(v), final = return_state ? state_like(q) : at::Tensor();
+    const at::Tensor states = bytes_like(q, cott_gated_scan_states_bytes(B, H, N, D, code)),
+                     ws = bytes_like(q, cott_gated_scan_workspace_bytes(B, H, N, D, code, 0));
+    cott_gated_layout lay = {};
+    lay.q = strides3(q), lay.k = strides3(k), lay.v = strides3(v), lay.out = strides3(out), lay.gate = strides3(gate);
+    check(cott_gated_scan_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), gate.data_ptr(), u8(kp), f32_or_null(init), out.data_ptr(),
+                              return_state ? final.data_ptr<float>() : nullptr, states.data_ptr(), ws.data_ptr(), &lay, B, H, N, D, code,
+                              dtype_code(gate.scalar_type()), stream_of(q)),
+          "cott_gated_scan_fwd");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, gate});
+    ctx->saved_data["states"] = states;
+    ctx->saved_data["with_initial"] = has(init);
+    ctx->saved_data["want_dinitial"] = want_dinitial;
+    save_opt(ctx, "keep", kp);
+    return return_state ? variable_list{out, final} : variable_list{out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(s[2]);
+    const OptTensor dfinal = grads.size() > 1 && grads[1].defined() ? OptTensor(grads[1]) : OptTensor(), keep = load_opt(ctx, "keep");
+    const at::Tensor states = ctx->saved_data["states"].toTensor();
+    const bool with_initial = ctx->saved_data["with_initial"].toBool(), want = ctx->saved_data["want_dinitial"].toBool();
+    Grads g;
+    if (at::GradMode::is_enabled()) {  // create_graph: through the dispatcher, which says that there is no second derivative
+      static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("cottention_b200::gated_bwd", "").typed<decltype(gated_bwd)>();
+      g = op.call(s[0], s[1], s[2], s[3], keep, with_initial, states, dout, dfinal, want);
+    } else {
+      g = gated_bwd(s[0], s[1], s[2], s[3], keep, with_initial, states, dout, dfinal, want);
+    }
+    auto& [dq, dk, dv, dg, dinit] = g;
+    return {dq, dk, dv, dg, Variable(), want ? dinit : Variable(), Variable(), Variable()};
+  }
+};
+variable_list gated_scan(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay, const OptTensor& keep,
+                         const OptTensor& initial, bool return_state) {
+  check_gated("gated_scan", q, k, v, log_decay);
+  if (has(initial)) check_gated_state("initial_state", *initial, q);
+  return GatedFn::apply(q, k, v, log_decay, keep, initial, return_state,
+                        has(initial) && at::GradMode::is_enabled() && initial->requires_grad());
+}
+at::Tensor gated_step(const at::Tensor& state, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& log_decay) {
+  check_gated("gated_scan_step", q_, k_, v_, log_decay);
+  check_gated_state("state", state, q_);
+  TORCH_CHECK(state.is_contiguous() && reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0,
+              "the state is updated in place: it must be contiguous and 16-byte aligned");
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(state.requires_grad() || q_.requires_grad() || k_.requires_grad() || v_.requires_grad() || log_decay.requires_grad()),
+              "gated_scan_step is not differentiable: use gated_scan, or call it under torch.no_grad()");
+  const at::Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty_like(v);
+  cott_gated_layout lay = {};
+  lay.q = strides3(q), lay.k = strides3(k), lay.v = strides3(v), lay.out = strides3(out), lay.gate = strides3(log_decay);
+  check(cott_gated_step(state.data_ptr<float>(), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), out.data_ptr(), &lay, (int)q.size(0),
+                        (int)q.size(1), (int)q.size(2), (int)q.size(3), dtype_code(q.scalar_type()), dtype_code(log_decay.scalar_type()), stream_of(q)),
+        "cott_gated_step");
+  state.unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+// the rotary tables as the C side takes them
+struct Tables {
+  at::Tensor sin, cos;
+  cott_rotary_tables t = {};
+  bool there = false;
+  Tables(const OptTensor& s, const OptTensor& c, const at::Tensor& q) {
+    if (!has(s)) return;
+    auto dense = [&](const at::Tensor& x) { return dense16(x.scalar_type() == at::kFloat && x.device() == q.device() ? x : x.to(q.device(), at::kFloat)); };
+    sin = dense(*s), cos = dense(*c);
+    const int64_t B = q.size(0), N = q.size(2), D = q.size(3), rot = sin.dim() ? 2 * sin.size(-1) : 0;
+    TORCH_CHECK(sin.sizes() == cos.sizes() && (sin.dim() == 2 || sin.dim() == 3) && sin.size(-2) == N &&
+                    (sin.dim() == 2 || sin.size(0) == 1 || sin.size(0) == B),
+                "sin / cos must be [N, rot/2] or [B, N, rot/2]");
+    TORCH_CHECK(rot >= 8 && rot % 8 == 0 && rot <= D, "the rotary dim must be a multiple of 8 and at most the head dim (got ", rot, ", ", D, ")");
+    t = cott_rotary_tables{sin.data_ptr<float>(), cos.data_ptr<float>(), (int)rot, sin.dim() == 3 && sin.size(0) > 1 ? (long long)(N * rot / 2) : 0};
+    there = true;
+  }
+  const cott_rotary_tables* get() const { return there ? &t : nullptr; }
+};
+using NormGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+NormGrads qk_norm_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const OptTensor& sin, const OptTensor& cos,
+                      const at::Tensor& dq_out_, const at::Tensor& dk_out_, double eps) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tables tab(sin, cos, q);
+  auto grad = [&](const at::Tensor& g) { return rows16(g.scalar_type() == q.scalar_type() ? g : g.to(q.scalar_type())); };
+  const at::Tensor dq_out = grad(dq_out_), dk_out = grad(dk_out_);
+  at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dqw = at::empty_like(qw), dkw = at::empty_like(kw);
+  const int B = (int)q.size(0), Hq = (int)q.size(1), Hk = (int)k.size(1), N = (int)q.size(2), D = (int)q.size(3);
+  const at::Tensor ws = bytes_like(q, cott_qk_norm_workspace_bytes(B, Hq, Hk, N, D));
+  const cott_norm_layout lay = {strides3(q), strides3(k), strides3(dq_out), strides3(dk_out), strides3(dq), strides3(dk)};
+  check(cott_qk_norm_bwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), tab.get(), dq_out.data_ptr(), dk_out.data_ptr(), ws.data_ptr(),
+                         dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), &lay, B, Hq, Hk, N, D, (float)eps, dtype_code(q.scalar_type()),
+                         dtype_code(qw.scalar_type()), stream_of(q)),
+        "cott_qk_norm_bwd");
+  return {dq, dk, dqw, dkw};
+}
+struct QKNormFn : torch::autograd::Function<QKNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& qw_, const at::Tensor& kw_,
+                               const OptTensor& sin, const OptTensor& cos, double eps) {
+    const at::Tensor q = rows16(q_), k = rows16(k_), qw = qw_.contiguous(), kw = kw_.contiguous();
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Tables tab(sin, cos, q);
+    at::Tensor q_out = at::empty_like(q), k_out = at::empty_like(k);
+    cott_norm_layout lay = {};
+    lay.q = strides3(q), lay.k = strides3(k), lay.q_out = strides3(q_out), lay.k_out = strides3(k_out);
+    check(cott_qk_norm_fwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), tab.get(), q_out.data_ptr(), k_out.data_ptr(), &lay, (int)q.size(0),
+                           (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)q.size(3), (float)eps, dtype_code(q.scalar_type()),
+                           dtype_code(qw.scalar_type()), stream_of(q)),
+          "cott_qk_norm_fwd");
+    ctx->save_for_backward({q, k, qw, kw, tab.sin, tab.cos});
+    ctx->saved_data["eps"] = eps;
+    return {q_out, k_out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const OptTensor sin = s[4].defined() ? OptTensor(s[4]) : OptTensor(), cos = s[5].defined() ? OptTensor(s[5]) : OptTensor();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    NormGrads g;
+    if (at::GradMode::is_enabled()) {
+      static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("cottention_b200::qk_norm_bwd", "").typed<decltype(qk_norm_bwd)>();
+      g = op.call(s[0], s[1], s[2], s[3], sin, cos, grads[0], grads[1], eps);
+    } else {
+      g = qk_norm_bwd(s[0], s[1], s[2], s[3], sin, cos, grads[0], grads[1], eps);
+    }
+    auto& [dq, dk, dqw, dkw] = g;
+    return {dq, dk, dqw, dkw, Variable(), Variable(), Variable()};
+  }
+};
+variable_list qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const OptTensor& sin,
+                             const OptTensor& cos, double eps) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && qw.is_cuda() && kw.is_cuda(), "qk_norm_rotary needs CUDA tensors (there is no CPU path)");
+  if (q.dim() != 4 || k.dim() != 4)
+    throw py::value_error("[B, H, N, D] tensors expected, got " + std::to_string(q.dim()) + " and " + std::to_string(k.dim()) + " dimensions");
+  const at::ScalarType t = q.scalar_type();
+  TORCH_CHECK((t == at::kFloat || t == at::kHalf || t == at::kBFloat16) && k.scalar_type() == t,
+              "qk_norm_rotary takes float32, float16 or bfloat16 tensors of one type, got ", t, " and ", k.scalar_type());
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3), "q and k must agree in all but their heads, got ", q.sizes(),
+              " and ", k.sizes());
+  const int64_t D = q.size(3);
+  TORCH_CHECK(D == 32 || D == 64 || D == 128, "qk_norm_rotary supports head dims 32, 64 and 128 (got ", D, ")");
+  for (const at::Tensor& w : {qw, kw})
+    TORCH_CHECK(w.sizes() == at::IntArrayRef({D}) && (w.scalar_type() == at::kFloat || w.scalar_type() == t) && w.scalar_type() == qw.scalar_type(),
+                "the weights must be [D] = [", D, "], both in float32 or both of the tensors' type, got ", w.sizes(), " in ", w.scalar_type());
+  TORCH_CHECK(k.device() == q.device() && qw.device() == q.device() && kw.device() == q.device(), "q, k and the weights must be on one device");
+  return QKNormFn::apply(q, k, qw, kw, sin, cos, eps);
+}
+
 // what Python calls
 at::Tensor cos_attn_causal(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& norm_const, const OptTensor& keep,
                            int64_t nseg, bool one_pass) {
@@ -555,6 +770,8 @@ TORCH_LIBRARY(cottention_b200, m) {
   m.def("causal_fwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, int nseg, bool save_states) -> (Tensor, Tensor, Tensor)");
   m.def("causal_bwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, Tensor dout, Tensor ws, Tensor saved, int nseg) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("bidir_fwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep) -> (Tensor, Tensor)");
+  m.def("gated_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? keep, bool with_initial, Tensor states, Tensor dout, Tensor? dfinal, bool want_dinitial) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("qk_norm_bwd(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor? sin, Tensor? cos, Tensor dq_out, Tensor dk_out, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("bidir_bwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, Tensor dout, Tensor scratch) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(cottention_b200, CUDA, m) {
@@ -562,6 +779,8 @@ TORCH_LIBRARY_IMPL(cottention_b200, CUDA, m) {
   m.impl("causal_bwd", &causal_bwd);
   m.impl("bidir_fwd", &bidir_fwd);
   m.impl("bidir_bwd", &bidir_bwd);
+  m.impl("gated_bwd", &gated_bwd);
+  m.impl("qk_norm_bwd", &qk_norm_bwd);
 }
 
 // The reference registers its four functions with pybind (combined_kernel_general.cu:444-454); the argument names and
@@ -580,6 +799,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("custom_attention", &custom_attention, Unlocked());
   m.def("decode_steps", &decode_steps, Unlocked());
   m.def("prefill", &prefill, Unlocked());
+  m.def("gated_scan", &gated_scan, Unlocked());
+  m.def("gated_step", &gated_step, Unlocked());
+  m.def("qk_norm_rotary", &qk_norm_rotary, Unlocked());
   m.def("float32", &forward_<at::kBFloat16>, "FastAttention forward (float32 entry point)", py::arg("Q"), py::arg("K"), py::arg("V"),
         py::arg("block_size"), py::arg("inplace") = false, py::arg("reversed") = false);
   m.def("float64", &forward_<at::kBFloat16>, "FastAttention forward (float64 entry point)", py::arg("Q"), py::arg("K"), py::arg("V"),

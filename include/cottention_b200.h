@@ -415,6 +415,68 @@ int cott_cos_attn_bwd_rotary(const void* q, const void* k, const void* v, const 
                              const cott_rotary_tables* rotary, void* dq, void* dk, void* dv, float* dnorm_const,
                              int B, int H, int N, int Dk, int Dv, int dtype, void* stream);
 
+/* ---- gated causal scan --------------------------------------------------------------------------------------
+ * The causal scan with a learned decay, per (batch, head) and position:
+ *     S_t = e^(log_decay_t) S_(t-1) + k_t v_t^T          out_t = S_t^T q_t
+ * q, k, v, out: [B, H, N, D], D = 32, 64 or 128; float32, float16 or bfloat16.  log_decay: [B, H, N], float32 or of the
+ * tensors' type, values <= 0; -inf drops the state (a document begins).  keep: NULL or [B, N] bytes, 0 = masked: such a
+ * position contributes nothing, lets the state pass unchanged, and its output and gradients are zero.
+ * initial_state, final_state and their gradients: NULL or fp32 [B, H, D, D], value index first (the layout of the decode
+ * state); initial_state may be final_state.
+ * The states before the chunks go from the forward to the backward in `states` (cott_gated_scan_states_bytes, 16-byte
+ * aligned); the backward reads them only, so it may run more than once.  `workspace`: cott_gated_scan_workspace_bytes of
+ * the direction, 16-byte aligned, may be NULL where that is 0; its contents mean nothing between calls.
+ * Rows are read and written 16 bytes at a time: base pointers and strides in multiples of 16 bytes (log_decay: any).
+ * Sums and states are fp32.  At head dims 64 and 128 the 16-bit types run on the tensor cores: the decayed scores of a
+ * chunk and the copy of a state that multiplies rows are rounded to the 16-bit type.  fp32 is fp32 throughout.
+ * NULL layout: dense [B, H, N, D] and [B, H, N]. */
+typedef struct cott_strides {
+  long long b, h, n; /* elements from one batch entry, head, position to the next; the innermost dimension is contiguous */
+} cott_strides;
+typedef struct cott_gated_layout {
+  cott_strides q, k, v;
+  cott_strides out;        /* of out; in the backward of dout */
+  cott_strides gate;       /* of log_decay */
+  cott_strides dq, dk, dv; /* read by the backward only */
+  cott_strides dgate;
+} cott_gated_layout;
+size_t cott_gated_scan_states_bytes(int B, int H, int N, int D, int dtype);
+size_t cott_gated_scan_workspace_bytes(int B, int H, int N, int D, int dtype, int backward);
+int cott_gated_scan_fwd(const void* q, const void* k, const void* v, const void* log_decay, const unsigned char* keep,
+                        const float* initial_state, void* out, float* final_state, void* states, void* workspace,
+                        const cott_gated_layout* layout, int B, int H, int N, int D, int dtype, int gate_dtype, void* stream);
+/* with_initial_state: whether the forward had one.  dfinal_state: NULL where the final state was not used.  dinitial_state:
+ * NULL where it is not wanted.  None of the outputs may overlap an input. */
+int cott_gated_scan_bwd(const void* q, const void* k, const void* v, const void* log_decay, const unsigned char* keep,
+                        int with_initial_state, const void* states, const void* dout, const float* dfinal_state, void* workspace,
+                        void* dq, void* dk, void* dv, void* dlog_decay, float* dinitial_state, const cott_gated_layout* layout,
+                        int B, int H, int N, int D, int dtype, int gate_dtype, void* stream);
+/* T consecutive tokens of the same recurrence on the fp32 states [B, H, D, D] (value index first), in place; q, k, v, out:
+ * [B, H, T, D], log_decay: [B, H, T].  out may not overlap q, k or v. */
+int cott_gated_step(float* state, const void* q, const void* k, const void* v, const void* log_decay, void* out,
+                    const cott_gated_layout* layout, int B, int H, int T, int D, int dtype, int gate_dtype, void* stream);
+
+/* ---- RMS norm of the heads of q and k, and the rotary embedding, in one pass -------------------------------------
+ *     n = x rsqrt(mean x^2 + eps)      y = Rot(n w)
+ * q: [B, Hq, N, D], k: [B, Hk, N, D], D = 32, 64 or 128; float32, float16 or bfloat16; q_weight, k_weight: [D], float32 or
+ * of the tensors' type.  rotary: NULL for none, else as for cott_rotary, rot_dim a multiple of 8.  Base pointers and
+ * strides in multiples of 16 bytes.  q_out may be q and k_out may be k (with the same strides).  NULL layout: dense.
+ * Backward: the gradients of q, k and of the weights (of the weights' type, summed in fp32 in a fixed order); dq may be
+ * dq_out and dk may be dk_out.  workspace: cott_qk_norm_workspace_bytes on the device that the call runs on. */
+typedef struct cott_norm_layout {
+  cott_strides q, k;
+  cott_strides q_out, k_out; /* of the results; in the backward of their gradients */
+  cott_strides dq, dk;       /* read by the backward only */
+} cott_norm_layout;
+int cott_qk_norm_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const cott_rotary_tables* rotary,
+                     void* q_out, void* k_out, const cott_norm_layout* layout, int B, int Hq, int Hk, int N, int D, float eps,
+                     int dtype, int weight_dtype, void* stream);
+size_t cott_qk_norm_workspace_bytes(int B, int Hq, int Hk, int N, int D);
+int cott_qk_norm_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const cott_rotary_tables* rotary,
+                     const void* dq_out, const void* dk_out, void* workspace, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                     const cott_norm_layout* layout, int B, int Hq, int Hk, int N, int D, float eps, int dtype, int weight_dtype,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif
