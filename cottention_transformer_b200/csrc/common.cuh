@@ -140,5 +140,8 @@ int launch_bidir_fwd_tc(const void* q, const void* k, const void* v, const unsig
 int launch_bidir_bwd_tc(const void* q, const void* k, const void* v, const unsigned char* keep, const float* nc,
                         const void* dout, void* dq, void* dk, void* dv, float* dnorm, int B, int H, int N, int dtype,
                         cudaStream_t stream, const cott_layout* layout = nullptr);
+// The status word of the gated scan's tensor-core kernels (a translation unit of their own): the code of the first device-side
+// wait that gave up, which is cleared.
+int gated_tc_status(int* value);
 
 }  // namespace cott

@@ -1195,10 +1195,16 @@ int cott_check_status(int* detail) {
   int v = 0;
   COTT_CUDA_TRY(cudaDeviceSynchronize());
   COTT_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_cott_status, sizeof(int)));
-  if (detail) *detail = v;
   if (v != 0) {
     int zero = 0;
     COTT_CUDA_TRY(cudaMemcpyToSymbol(g_cott_status, &zero, sizeof(int)));
+  }
+  int of_gated = 0;  // the gated kernels are a translation unit of their own, with a status word of their own
+  const int st = gated_tc_status(&of_gated);
+  if (st) return st;
+  if (v == 0) v = of_gated;
+  if (detail) *detail = v;
+  if (v != 0) {
     return fail(COTT_ERR_DEVICE_WAIT, "a device-side wait gave up: stage %d (1=TMA, 2=score MMA, 3=accumulator MMA) at chunk %d",
                 v >> 16, v & 0xffff);
   }

@@ -107,11 +107,14 @@ extern "C" {
 
 size_t cott_gated_scan_states_bytes(int B, int H, int N, int D, int dtype) {
   if (B <= 0 || H <= 0 || N <= 0 || check_sizes("cott_gated_scan", B, H, N, D, dtype, COTT_F32)) return 0;
+  if (gated_tc_usable(D, dtype)) return gated_tc_states_bytes(B, H, N, D);
   return prefix_floats(B, H, N, D) * sizeof(float) + round16((size_t)B * H * chunks_of(N) * sizeof(float));
 }
 
 size_t cott_gated_scan_workspace_bytes(int B, int H, int N, int D, int dtype, int backward) {
-  if (B <= 0 || H <= 0 || N <= 0 || check_sizes("cott_gated_scan", B, H, N, D, dtype, COTT_F32) || !backward) return 0;
+  if (B <= 0 || H <= 0 || N <= 0 || check_sizes("cott_gated_scan", B, H, N, D, dtype, COTT_F32)) return 0;
+  if (gated_tc_usable(D, dtype)) return gated_tc_workspace_bytes(B, H, N, D, backward != 0);
+  if (!backward) return 0;
   return (suffix_floats(B, H, N, D) + 2 * (size_t)B * H * chunks_of(N) * kGsChunk) * sizeof(float);
 }
 
@@ -120,7 +123,6 @@ int cott_gated_scan_fwd(const void* q, const void* k, const void* v, const void*
                         int dtype, int gate_dtype, void* stream) {
   int st = check_sizes("cott_gated_scan_fwd", B, H, N, D, dtype, gate_dtype);
   if (st) return st;
-  (void)workspace;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long n = (long)B * H;
   if ((st = check_state("initial_state", initial_state)) || (st = check_state("final_state", final_state))) return st;
@@ -146,6 +148,11 @@ int cott_gated_scan_fwd(const void* q, const void* k, const void* v, const void*
   COTT_CUDA_TRY(scope.status());
   g.q = q, g.k = k, g.v = v, g.gate = log_decay, g.keep = keep, g.initial = initial_state, g.out = out, g.final_state = final_state;
   g.with_initial = initial_state != nullptr;
+  if (gated_tc_usable(D, dtype)) {
+    if (!workspace && gated_tc_workspace_bytes(B, H, N, D, false)) return fail(COTT_ERR_NULL, "null pointer: workspace");
+    if ((st = check_state("workspace", workspace))) return st;
+    return gated_tc_fwd(g, states, workspace, B, D, dtype, s);
+  }
   g.prefix = static_cast<float*>(states), g.total = g.prefix + prefix_floats(B, H, N, D);
   return run_any<true>(g, D, dtype, n, s);
 }
@@ -182,6 +189,7 @@ int cott_gated_scan_bwd(const void* q, const void* k, const void* v, const void*
   COTT_CUDA_TRY(scope.status());
   g.q = q, g.k = k, g.v = v, g.dout = dout, g.gate = log_decay, g.keep = keep, g.dfinal = dfinal_state, g.dinitial = dinitial_state;
   g.dq = dq, g.dk = dk, g.dv = dv, g.dgate = dlog_decay, g.with_initial = with_initial_state != 0;
+  if (gated_tc_usable(D, dtype)) return gated_tc_bwd(g, states, workspace, B, D, dtype, s);
   g.prefix = const_cast<float*>(static_cast<const float*>(states)), g.total = g.prefix + prefix_floats(B, H, N, D);
   g.suffix = static_cast<float*>(workspace), g.qdot = g.suffix + suffix_floats(B, H, N, D), g.kdot = g.qdot + (size_t)n * g.nchunks * kGsChunk;
   return run_any<false>(g, D, dtype, n, s);

@@ -121,8 +121,8 @@ __device__ __forceinline__ void gs_stage(float* dst, const void* src, const Gate
 template <typename T, int D, bool REV>
 __global__ void __launch_bounds__(kGsThreads) gated_state_kernel(const GatedArgs g) {
   constexpr int NB = D / 16, LD = D + 4;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* sY = reinterpret_cast<float*>(smem_raw);
+  extern __shared__ __align__(16) unsigned char gs_smem[];
+  float* sY = reinterpret_cast<float*>(gs_smem);
   float* sZ = sY + kGsChunk * LD;
   __shared__ double G[kGsChunk];
   __shared__ float w[kGsChunk];
@@ -374,8 +374,8 @@ __device__ __forceinline__ void gated_chunk(const GatedArgs& g, float* sA, float
 // FWD: grid = B*H * chunks.  Backward: grid = (B*H * chunks, 3), y = dq, dk, dv.
 template <typename T, int D, bool FWD>
 __global__ void __launch_bounds__(kGsThreads, D > 64 ? 1 : 2) gated_chunk_kernel(const GatedArgs g) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* sA = reinterpret_cast<float*>(smem_raw);
+  extern __shared__ __align__(16) unsigned char gs_smem[];
+  float* sA = reinterpret_cast<float*>(gs_smem);
   float* sB = sA + kGsChunk * (D + 4);
   float* sC = sB + kGsChunk * (D + 4);
   float* sP = sC + kGsChunk * (D + 4);
@@ -447,5 +447,12 @@ __global__ void __launch_bounds__(kGsThreads) gated_dgate_kernel(const GatedArgs
     }
   }
 }
+
+// The tensor-core kernels of the 16-bit types at head dims 64 and 128 (gated_tc_api.cu); `states`, `workspace` as in the C ABI.
+bool gated_tc_usable(int D, int dtype);
+size_t gated_tc_states_bytes(int B, int H, int N, int D);
+size_t gated_tc_workspace_bytes(int B, int H, int N, int D, bool backward);
+int gated_tc_fwd(const GatedArgs& g, void* states, void* workspace, int B, int D, int dtype, cudaStream_t stream);
+int gated_tc_bwd(const GatedArgs& g, const void* states, void* workspace, int B, int D, int dtype, cudaStream_t stream);
 
 }  // namespace cott
