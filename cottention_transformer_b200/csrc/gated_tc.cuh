@@ -5,12 +5,10 @@
 //                       (backwards: R <- A R + Q^T diag(e^(G_t)) dO), and leaves the state before (after) every chunk in memory as
 //                       the 16-bit operand that the other kernel wants.  The weighted operand is split into a 16-bit head and a
 //                       16-bit tail, two MMAs, so that a state is exact to about 2^-17: it lasts for the rest of the sequence.
-//   gated_chunk_tc      one CTA per chunk and 64 columns of the result, none of which waits for another:
-//                           P   = A B^T           128 x 128 x D      scores, decayed, masked and rounded to 16 bits in registers
-//                           acc = A M             128 x 64 x D       the state's part, scaled by the row factor in fp32
-//                           acc += P C            128 x 64 x 128     P as the A operand from TMEM
-//                       with (A, B, C, M) = (q, k, v, S) for out, (dO, v, k, S^T) for dq, (v, dO, q, R^T) for dk, (k, q, dO, R) for dv.
-// HBM-bound: the walk reads two tensors and writes half of one, the chunks read three (four and two states backwards).
+//   gated_fwd_tc_kernel, gated_bwd_tc_kernel   one CTA per chunk, none of which waits for another: scores by MMA, decayed, masked and
+//                       rounded to 16 bits in registers, back to TMEM as the A operand of the product with the rows; the state's part in
+//                       fp32, scaled by the row factor, beside it.
+// HBM-bound: the walk reads two tensors and writes half of one, the chunks read three and half of one, backwards four and a whole.
 //
 // The decays of a chunk: D_ts = e^(G_t - G_s) of the 32 x 32 blocks on the diagonal are taken element by element; a block below it
 // is the product of a row factor e^(G_t - G_b) and a column factor e^(G_b - G_s) with b the last position before the block's
@@ -25,8 +23,7 @@ namespace cott {
 
 constexpr int kGtChunk = 128;
 constexpr int kStateTile = 64 * 128;      // bytes of a [64 x 64] 16-bit tile
-constexpr int kWalkThreads = 320;
-constexpr int kGtThreads = 256;
+constexpr int kWalkThreads = 448;
 constexpr float kGateFloorTc = -200.f;    // e^-200 = 0 in fp32; sums of it keep their digits
 
 enum { kWaitWalkTma = 16, kWaitWalkFree = 17, kWaitWalkPrep = 18, kWaitWalkState = 19, kWaitChunkTma = 20, kWaitChunkMma = 21 };
@@ -37,7 +34,7 @@ struct GatedTcArgs {
   cott_strides sg;
   const float* edge;        // [B*H][value][key]: the state before the walk's first chunk, or null
   float* last;              // [B*H][value][key]: the state after its last one, or null
-  unsigned char* states;    // [B*H][nchunks][D/64][D/64] swizzled tiles; c: before chunk c (REV: after it)
+  unsigned char* states;    // [B*H][nchunks][D/64] swizzled [D x 64] panels (key x value); c: before chunk c (REV: after it)
   float* seg_state;         // [B*H][D/64][segments][D][64]: sums of the segments, then the states before them
   float* seg_log;           // [B*H][segments]
   int H, N, nchunks, chunks_per_seg, nseg, gate_f32;
@@ -116,7 +113,8 @@ template <int D, int SPLIT> constexpr size_t walk_smem() { return 1024 + walk_st
 // grid = (B*H, segments, D/64): one CTA owns 64 value columns of a segment's state.  Y = K, Z = V, or REV: Y = Q, Z = dO and the
 // chunks and segments are numbered from the end of the sequence.  EMIT: starts from the segment's state and leaves the state
 // before every chunk; else it sums the segment up, from zero.
-//   warps 0-3: state (fp32, in registers: a row of it per thread)    warps 4-7: weighted operand    warp 8: TMA    warp 9: MMA
+//   warps 0-3: state (fp32, in registers: a row of it per thread)    warp 8: TMA    warp 9: MMA
+//   warps 4-7, 10-13: weighted operand of the even / odd chunks
 // SPLIT: into how many 16-bit numbers the weighted operand is split.  Two where the states are wanted as 16-bit operands, three
 // where the last one is a result: it is then what fp32 products give.
 template <typename T, int D, bool REV, bool EMIT, int SPLIT>
@@ -157,8 +155,9 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     tma_prefetch_desc(&mapY);
     tma_prefetch_desc(&mapZ);
   }
+  constexpr uint32_t kUCols = 64 * SPLIT, kCols = SPLIT == 2 ? 256 : 512;  // the parts of the operand side by side: one MMA, summed when read
   if (warp == 9) {
-    tmem_alloc(&tmem_slot, 128);
+    tmem_alloc(&tmem_slot, kCols);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -182,7 +181,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     }
   } else if (warp == 9) {
     if (elect_one()) {
-      constexpr uint32_t kIdesc = make_idesc(D, 64, BF, true, true);
+      constexpr uint32_t kIdesc = make_idesc(D, kUCols, BF, true, true);
       for (int c = 0; c < updates; ++c) {
         const int s = c % NS, u = c & 1;
         if (!wait_bar2(&bar_prep[s], (c / NS) & 1, c >= 2 ? &bar_u_free[u] : &bar_prep[s], c >= 2 ? ((c >> 1) - 1) & 1 : (c / NS) & 1, abort_flag,
@@ -190,20 +189,16 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
           break;
         tc_fence_after_sync();
         const uint32_t st = smem_u32(smem + s * STAGE);
-        const uint64_t dY = make_smem_desc(st, kTileBytes, 1024);
+        const uint64_t dY = make_smem_desc(st, kTileBytes, 1024), dZ = make_smem_desc(st + NT * kTileBytes, kTileBytes, 1024);
 #pragma unroll
-        for (int i = 0; i < SPLIT; ++i) {
-          const uint64_t dZ = mdesc(st + (NT + i) * kTileBytes);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) mma_ss(tU + 64 * u, dY + 128 * k, dZ + 128 * k, kIdesc, i > 0 || k > 0);
-        }
+        for (int k = 0; k < 8; ++k) mma_ss(tU + kUCols * u, dY + 128 * k, dZ + 128 * k, kIdesc, k > 0);
         mma_commit(&bar_free[s]);
         mma_commit(&bar_u_full[u]);
       }
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- weighted operand
-    const int wq = warp & 3, row = 32 * wq + lane;
+    const int wq = warp & 3, row = 32 * wq + lane, mine = warp >= 10 ? 1 : 0;
     float g[4];
     bool kp = true;
     auto fetch = [&](int c) {
@@ -212,9 +207,13 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, p0 + 4 * lane + e);
       kp = !a.keep || (p0 + row < a.N && a.keep[b * a.N + p0 + row]);
     };
-    if (updates > 0) fetch(0);
+    if (updates > mine) fetch(mine);
     for (int c = 0; c < updates; ++c) {
       const int s = c % NS;
+      if ((c & 1) != mine) {  // every phase of a barrier has to be seen: a parity cannot tell a phase from the next but one
+        if (!wait_bar_warp(&bar_full[s], (c / NS) & 1, abort_flag, kWaitWalkTma, c)) break;
+        continue;
+      }
       gate_sums<!REV>(g, lane);  // G_last - G_s, or G_t
       float G = 0.f;
 #pragma unroll
@@ -224,7 +223,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       }
       const float w = __expf(G);
       const bool take = kp;
-      if (c + 1 < updates) fetch(c + 1);
+      if (c + 2 < updates) fetch(c + 2);
       if (!wait_bar_warp(&bar_full[s], (c / NS) & 1, abort_flag, kWaitWalkTma, c)) break;
       unsigned char *sY = smem + s * STAGE, *sZ = sY + NT * kTileBytes;
       if (take) {
@@ -271,8 +270,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, p0 + 4 * lane + e);
     };
     auto emit = [&](int slot, int n) {  // n: how many were emitted before
-      unsigned char* tile = sOut + ((n & 1) * NT + (D == 128 ? wq >> 1 : 0)) * kStateTile;
-      const int r = i & 63;
+      unsigned char* panel = sOut + (n & 1) * NT * kStateTile;
       if (lane == 0) tma_store_wait_read<1>();  // the copy of two emissions ago has left the buffer
       __syncwarp();
       if (mine) {
@@ -281,16 +279,15 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
           uint4 u;
           u.x = Pack2<T>::pack(S[8 * j], S[8 * j + 1]), u.y = Pack2<T>::pack(S[8 * j + 2], S[8 * j + 3]);
           u.z = Pack2<T>::pack(S[8 * j + 4], S[8 * j + 5]), u.w = Pack2<T>::pack(S[8 * j + 6], S[8 * j + 7]);
-          *tile_piece(tile, r, j) = u;
+          *tile_piece(panel, i, j) = u;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         constexpr int ROWS = D == 64 ? 16 : 32;
-        const int r0 = (ROWS * wq) & 63;
-        unsigned char* dst = a.states + (((bh * a.nchunks + slot) * NT + (D == 128 ? wq >> 1 : 0)) * NT + J) * static_cast<long>(kStateTile);
-        bulk_store(dst + r0 * 128, tile + r0 * 128, ROWS * 128);
+        unsigned char* dst = a.states + ((bh * a.nchunks + slot) * NT + J) * static_cast<long>(NT * kStateTile);
+        bulk_store(dst + ROWS * wq * 128, panel + ROWS * wq * 128, ROWS * 128);
         tma_store_commit();
       }
     };
@@ -307,17 +304,22 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       if (c + 1 < updates) fetch(c + 1);
       if (!(ok = wait_bar_warp(&bar_u_full[c & 1], (c >> 1) & 1, abort_flag, kWaitWalkState, c))) break;
       tc_fence_after_sync();
-      uint32_t r[32];
+      if (A == 0.f) {  // a state that is dropped is dropped whatever it holds
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        tmem_ld_x32(tU + 64 * (c & 1) + 32 * half + lane_base, r);
+        for (int j = 0; j < 64; ++j) S[j] = 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // 16 columns at a time: more of them do not fit beside the state
+        uint32_t r[SPLIT][16];
+#pragma unroll
+        for (int i = 0; i < SPLIT; ++i) tmem_ld_x16(tU + kUCols * (c & 1) + 64 * i + 16 * q + lane_base, r[i]);
         tmem_ld_wait();
-        if (A == 0.f) {  // a state that is dropped is dropped whatever it holds
 #pragma unroll
-          for (int j = 0; j < 32; ++j) S[32 * half + j] = __uint_as_float(r[j]);
-        } else {
+        for (int j = 0; j < 16; ++j) {
+          float x = __uint_as_float(r[SPLIT - 1][j]);  // the smallest parts first
 #pragma unroll
-          for (int j = 0; j < 32; ++j) S[32 * half + j] = fmaf(A, S[32 * half + j], __uint_as_float(r[j]));
+          for (int i = SPLIT - 2; i >= 0; --i) x += __uint_as_float(r[i][j]);
+          S[16 * q + j] = fmaf(A, S[16 * q + j], x);
         }
       }
       tc_fence_before_sync();
@@ -343,7 +345,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     for (int c = updates > NS ? updates - NS : 0; c < updates; ++c) mbar_wait(&bar_full[c % NS], (c / NS) & 1, 64);
   }
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tU, 128);
+  if (warp == 9) tmem_dealloc(tU, kCols);
 }
 
 // The states before the segments, in place of their sums: run <- e^(log) run + sum.  grid = (B*H * D/64, D * 64 / 256).
@@ -375,52 +377,141 @@ __global__ void __launch_bounds__(256) gated_seg_kernel(const GatedTcArgs a) {
 struct GatedChunkArgs {
   const void* gate;
   const unsigned char* keep;
-  cott_strides sg;
-  const unsigned char *S, *R;          // [B*H][nchunks] state tiles: before, after a chunk
-  const void *q, *k;                   // for the products with dq and dk
-  cott_strides sq, sk;
-  float *qdot, *kdot, *bdot;           // [D/64][B*H][nchunks][128]: q.dq; k.dk within the chunk and across its end
-  long units;                          // B*H * nchunks
+  cott_strides sg, sdg;
+  const unsigned char *S, *R;  // [B*H][nchunks] states: before, after a chunk
+  void* dgate;
+  long units;                  // B*H * nchunks
   int H, N, nchunks, gate_f32, with_first, with_last;  // a state before the first chunk, a gradient after the last one
 };
-struct GatedMaps {
-  CUtensorMap q, k, v, o, dq, dk, dv;  // o: out, or dO
-};
-template <int D> constexpr int chunk_tc_bytes() { return 2 * (D / 64) * kTileBytes + kTileBytes + (D / 64) * kStateTile; }
-template <int D> constexpr size_t chunk_tc_smem() { return 1024 + chunk_tc_bytes<D>(); }
 
-// One pass (kGsOut, kGsDq, kGsDk, kGsDv) over one chunk and one 64-column slice J of its result.
+// What the CTAs of both chunk kernels begin with: sums of the gates, and the column factors of the decays of the blocks off the
+// diagonal (LOWER: below it).
+template <typename T>
+__device__ __forceinline__ void chunk_gates(const GatedChunkArgs& a, float* sG, long b, int h, int c0, int lane) {
+  float g[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
+  gate_sums<false>(g, lane);
+  *reinterpret_cast<float4*>(&sG[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
+}
+template <bool LOWER>
+__device__ __forceinline__ void col_factor(float (*sCol)[kGtChunk], const float* sG, int w, int s) {
+  if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = __expf(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
+}
+// 32 columns (block `blk`) of the scores of a row of block wq, decayed, masked and packed
+template <typename T, bool LOWER>
+__device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_lane, int blk, int wq, int lane, float Gr, float rowf, const float* sG,
+                                            const float* col) {
+  if (LOWER ? blk > wq : blk < wq) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) pk[j] = 0u;
+    return;
+  }
+  uint32_t r[32];
+  ptx::tmem_ld_x32(taddr_lane + 32 * blk, r);
+  ptx::tmem_ld_wait();
+  if (blk == wq) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 Gs = *reinterpret_cast<const float4*>(&sG[32 * blk + j]);
+      const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = LOWER ? j + e <= lane : j + e >= lane;
+        x[e] = in ? __uint_as_float(r[j + e]) * __expf(LOWER ? Gr - gs[e] : gs[e] - Gr) : 0.f;
+      }
+      pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
+      pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 cf = *reinterpret_cast<const float4*>(&col[32 * blk + j]);
+      pk[j / 2] = Pack2<T>::pack(__uint_as_float(r[j]) * (rowf * cf.x), __uint_as_float(r[j + 1]) * (rowf * cf.y));
+      pk[j / 2 + 1] = Pack2<T>::pack(__uint_as_float(r[j + 2]) * (rowf * cf.z), __uint_as_float(r[j + 3]) * (rowf * cf.w));
+    }
+  }
+}
+// 32 columns of an accumulator, scaled by f (0: whatever they hold)
+__device__ __forceinline__ void acc_scaled(float (&acc)[32], uint32_t taddr_lane, float f) {
+  uint32_t r[32];
+  ptx::tmem_ld_x32(taddr_lane, r);
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[j] = f == 0.f ? 0.f : f * __uint_as_float(r[j]);
+}
+__device__ __forceinline__ void acc_add(float (&acc)[32], uint32_t taddr_lane) {
+  uint32_t r[32];
+  ptx::tmem_ld_x32(taddr_lane, r);
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) acc[j] += __uint_as_float(r[j]);
+}
+// 32 columns of a row -> pieces j0 .. j0 + 3 of a tile's row
+template <typename T>
+__device__ __forceinline__ void stage_row(unsigned char* tile, int row, int j0, const float (&acc)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 u;
+    u.x = Pack2<T>::pack(acc[8 * j], acc[8 * j + 1]), u.y = Pack2<T>::pack(acc[8 * j + 2], acc[8 * j + 3]);
+    u.z = Pack2<T>::pack(acc[8 * j + 4], acc[8 * j + 5]), u.w = Pack2<T>::pack(acc[8 * j + 6], acc[8 * j + 7]);
+    *tile_piece(tile, row, j0 + j) = u;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float row_dot32(unsigned char* tile, int row, int j0, const float (&acc)[32]) {
+  float d = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 p = *tile_piece(tile, row, j0 + j);
+    const uint32_t u[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = Pack2<T>::unpack(u[e]);
+      d = fmaf(f.x, acc[8 * j + 2 * e], fmaf(f.y, acc[8 * j + 2 * e + 1], d));
+    }
+  }
+  return d;
+}
+
+constexpr int kFwdThreads = 256;
+template <int D> constexpr size_t fwd_tc_smem() { return 1024 + 2 * (D / 64) * kTileBytes + kTileBytes + (D / 64) * kStateTile; }
+
+// Forward, one chunk and 64 columns J of the result; grid = B*H * chunks * D/64 (the CTAs of a chunk are neighbours: its q and k are
+// read from memory once).  Everything in a CTA is one chain; three CTAs per SM cover each other.
 //   warp w: TMEM lanes / rows 32 (w % 4) .., columns 64 (w / 4) .. of the scores and 32 (w / 4) .. of the accumulator
-template <typename T, int D, int PASS>
-__device__ __forceinline__ void gated_chunk_tc(const CUtensorMap& mapA, const CUtensorMap& mapB, const CUtensorMap& mapC, const CUtensorMap& mapO,
-                                               const GatedChunkArgs& a, const long unit, const int J) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kFwdThreads, D == 64 ? 3 : 2)
+gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                    const __grid_constant__ CUtensorMap mapO, const GatedChunkArgs a) {
   using namespace ptx;
   constexpr int NT = D / 64;
-  constexpr bool BF = Pack2<T>::kBf16, LOWER = PASS == kGsOut || PASS == kGsDq, MT = PASS == kGsDq || PASS == kGsDk;
+  constexpr bool BF = Pack2<T>::kBf16;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char *sA = smem, *sB = sA + NT * kTileBytes, *sC = sB + NT * kTileBytes, *sM = sC + kTileBytes;
+  unsigned char *sQ = smem, *sK = sQ + NT * kTileBytes, *sV = sK + NT * kTileBytes, *sS = sV + kTileBytes;
   __shared__ uint64_t bar_full, bar_mma[3];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
-  __shared__ __align__(16) float sG[kGtChunk], sCol[4][kGtChunk], sDot[2][kGtChunk];  // (read four at a time)
+  __shared__ __align__(16) float sG[kGtChunk], sCol[4][kGtChunk];  // (read four at a time)
   volatile int* abort_flag = &abort_flag_s;
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const int wq = warp & 3, hf = warp >> 2, row = 32 * wq + lane;
-  const long bh = unit / a.nchunks, b = bh / a.H;
+  const int wq = warp & 3, hf = warp >> 2, row = 32 * wq + lane, J = static_cast<int>(blockIdx.x % NT);
+  const long unit = blockIdx.x / NT, bh = unit / a.nchunks, b = bh / a.H;
   const int chunk = static_cast<int>(unit % a.nchunks), h = static_cast<int>(bh % a.H), c0 = chunk * kGtChunk;
-  const bool with_state = LOWER ? chunk > 0 || a.with_first : chunk + 1 < a.nchunks || a.with_last;
+  const bool with_state = chunk > 0 || a.with_first;
   const uint32_t lane_base = static_cast<uint32_t>(32 * wq) << 16;
   if (tid == 0) {
     mbar_init(&bar_full, 1);
     for (int i = 0; i < 3; ++i) mbar_init(&bar_mma[i], 1);
     mbar_fence_init();
     abort_flag_s = 0;
-    tma_prefetch_desc(&mapA);
-    tma_prefetch_desc(&mapB);
-    tma_prefetch_desc(&mapC);
+    tma_prefetch_desc(&mapQ);
+    tma_prefetch_desc(&mapK);
+    tma_prefetch_desc(&mapV);
     tma_prefetch_desc(&mapO);
   }
   if (warp == 1) {
@@ -439,193 +530,97 @@ __device__ __forceinline__ void gated_chunk_tc(const CUtensorMap& mapA, const CU
       mbar_expect_tx(&bar_full, (2 * NT + 1) * kTileBytes + (with_state ? NT * kStateTile : 0));
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        tma_load_tile_x(sA + i * kTileBytes, &mapA, &bar_full, 64 * i, c0, h, bi);
-        tma_load_tile_x(sB + i * kTileBytes, &mapB, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sQ + i * kTileBytes, &mapQ, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sK + i * kTileBytes, &mapK, &bar_full, 64 * i, c0, h, bi);
       }
-      tma_load_tile_x(sC, &mapC, &bar_full, 64 * J, c0, h, bi);
-      if (with_state) {
-        // out, dv: column J of the tiles of S, R; dq, dk: row J
-        const unsigned char* m = LOWER ? a.S + unit * (NT * NT * kStateTile) : a.R + unit * (NT * NT * kStateTile);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) bulk_load(sM + i * kStateTile, m + (MT ? J * NT + i : i * NT + J) * kStateTile, kStateTile, &bar_full);
-      }
+      tma_load_tile_x(sV, &mapV, &bar_full, 64 * J, c0, h, bi);
+      if (with_state) bulk_load(sS, a.S + (unit * NT + J) * (NT * kStateTile), NT * kStateTile, &bar_full);
     }
     __syncwarp();
   } else if (warp == 4) {
-    float g[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
-    gate_sums<false>(g, lane);
-    *reinterpret_cast<float4*>(&sG[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
+    chunk_gates<T>(a, sG, b, h, c0, lane);
   }
   const bool kp = !a.keep || (c0 + row < a.N && a.keep[b * a.N + c0 + row]);
   __syncthreads();
-  // column factors: of the rows of block w, relative to the boundary between them and the columns
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int w = 2 * i + (tid >> 7), s = tid & 127;
-    if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = __expf(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
-  }
+  for (int i = 0; i < 2; ++i) col_factor<true>(sCol, sG, 2 * i + (tid >> 7), tid & 127);
   if (a.keep) {  // nothing of a masked position gets into a product
     wait_bar_warp(&bar_full, 0, abort_flag, kWaitChunkTma, chunk);
     if (!kp) {
       const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int j = 4 * hf; j < 4 * hf + 4; ++j) {
-        for (int i = 0; i < 2 * NT; ++i) *tile_piece(sA + i * kTileBytes, row, j) = zero;
-        *tile_piece(sC, row, j) = zero;
-      }
+      for (int j = 4 * hf; j < 4 * hf + 4; ++j)
+        for (int i = 0; i < 2 * NT + 1; ++i) *tile_piece(sQ + i * kTileBytes, row, j) = zero;
     }
     fence_proxy_async_smem();
   }
   __syncthreads();
-  constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescM = make_idesc(128, 64, BF, false, !MT),
-                     kIdescC = make_idesc(128, 64, BF, false, true);
-  constexpr uint64_t kPanel = kTileBytes >> 4, kPanelM = kStateTile >> 4;
-  const uint64_t dA = kdesc(smem_u32(sA));
+  constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescAcc = make_idesc(128, 64, BF, false, true);
+  constexpr uint64_t kPanel = kTileBytes >> 4;
+  const uint64_t dQ = kdesc(smem_u32(sQ));
   if (warp == 0) {
     if (elect_one() && wait_bar1(&bar_full, 0, abort_flag, kWaitChunkTma, chunk)) {
       tc_fence_after_sync();
-      const uint64_t dB = kdesc(smem_u32(sB));
+      const uint64_t dK = kdesc(smem_u32(sK));
 #pragma unroll
-      for (int k = 0; k < 4 * NT; ++k) mma_ss(tP, dA + (k >> 2) * kPanel + 2 * (k & 3), dB + (k >> 2) * kPanel + 2 * (k & 3), kIdescP, k > 0);
+      for (int k = 0; k < 4 * NT; ++k) mma_ss(tP, dQ + (k >> 2) * kPanel + 2 * (k & 3), dK + (k >> 2) * kPanel + 2 * (k & 3), kIdescP, k > 0);
       mma_commit(&bar_mma[0]);
     }
     __syncwarp();
   }
-  // ---- the scores: this thread has 64 columns of its row
   wait_bar_warp(&bar_mma[0], 0, abort_flag, kWaitChunkMma, chunk);
   tc_fence_after_sync();
-  const float Gr = sG[row];
-  const float rowf = __expf(LOWER ? (wq > 0 ? Gr - sG[32 * wq - 1] : 0.f) : sG[32 * wq + 31] - Gr);
-  uint32_t pk[32];
+  const float Gr = sG[row], rowf = __expf(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f);
+  uint32_t pk[2][16];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int blk = 2 * hf + i;
-    if (LOWER ? blk > wq : blk < wq) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) pk[16 * i + j] = 0u;
-    } else {
-      uint32_t r[32];
-      tmem_ld_x32(tP + lane_base + 32 * blk, r);
-      tmem_ld_wait();
-      if (blk == wq) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 Gs = *reinterpret_cast<const float4*>(&sG[32 * blk + j]);
-          const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool in = LOWER ? j + e <= lane : j + e >= lane;
-            x[e] = in ? __uint_as_float(r[j + e]) * __expf(LOWER ? Gr - gs[e] : gs[e] - Gr) : 0.f;
-          }
-          pk[16 * i + j / 2] = Pack2<T>::pack(x[0], x[1]);
-          pk[16 * i + j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 cf = *reinterpret_cast<const float4*>(&sCol[wq][32 * blk + j]);
-          pk[16 * i + j / 2] = Pack2<T>::pack(__uint_as_float(r[j]) * (rowf * cf.x), __uint_as_float(r[j + 1]) * (rowf * cf.y));
-          pk[16 * i + j / 2 + 1] = Pack2<T>::pack(__uint_as_float(r[j + 2]) * (rowf * cf.z), __uint_as_float(r[j + 3]) * (rowf * cf.w));
-        }
-      }
-    }
-  }
-  uint4 x[4];
-  const bool dot_row = MT && kp && c0 + row < a.N;
-  if (dot_row) {
-    const cott_strides& sx = PASS == kGsDq ? a.sq : a.sk;
-    const T* p = static_cast<const T*>(PASS == kGsDq ? a.q : a.k) + b * sx.b + h * sx.h + static_cast<long long>(c0 + row) * sx.n + 64 * J + 32 * hf;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = reinterpret_cast<const uint4*>(p)[j];
-  }
-  auto dot_of = [&](const float (&y)[32]) {
-    float d = 0.f;
-    if (dot_row) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t u[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = Pack2<T>::unpack(u[e]);
-          d = fmaf(f.x, y[8 * j + 2 * e], fmaf(f.y, y[8 * j + 2 * e + 1], d));
-        }
-      }
-    }
-    return d;
-  };
+  for (int i = 0; i < 2; ++i) decay_block<T, true>(pk[i], tP + lane_base, 2 * hf + i, wq, lane, Gr, rowf, sG, sCol[wq]);
   tc_fence_before_sync();
   __syncthreads();  // all scores have been read: their columns become P (the first 64) and the accumulator
   if (with_state && warp == 0) {
     if (elect_one() && !*abort_flag) {
       tc_fence_after_sync();
-      const uint64_t dM = MT ? kdesc(smem_u32(sM)) : mdesc(smem_u32(sM));
+      const uint64_t dS = mdesc(smem_u32(sS));
 #pragma unroll
-      for (int k = 0; k < 4 * NT; ++k)
-        mma_ss(tAcc, dA + (k >> 2) * kPanel + 2 * (k & 3), MT ? dM + (k >> 2) * kPanelM + 2 * (k & 3) : dM + 128 * k, kIdescM, k > 0);
+      for (int k = 0; k < 4 * NT; ++k) mma_ss(tAcc, dQ + (k >> 2) * kPanel + 2 * (k & 3), dS + 128 * k, kIdescAcc, k > 0);
       mma_commit(&bar_mma[1]);
     }
     __syncwarp();
   }
   tc_fence_after_sync();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) tmem_st_x16(tP + lane_base + 32 * hf + 16 * i, pk + 16 * i);
+  for (int i = 0; i < 2; ++i) tmem_st_x16(tP + lane_base + 32 * hf + 16 * i, pk[i]);
   tmem_st_wait();
   float acc[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) acc[j] = 0.f;
   if (with_state) {
     wait_bar_warp(&bar_mma[1], 0, abort_flag, kWaitChunkMma, chunk);
     tc_fence_after_sync();
-    const float f = __expf(LOWER ? Gr : sG[kGtChunk - 1] - Gr);
-    uint32_t r[32];
-    tmem_ld_x32(tAcc + lane_base + 32 * hf, r);
-    tmem_ld_wait();
+    acc_scaled(acc, tAcc + lane_base + 32 * hf, __expf(Gr));
+  } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) acc[j] = f == 0.f ? 0.f : f * __uint_as_float(r[j]);
+    for (int j = 0; j < 32; ++j) acc[j] = 0.f;
   }
   tc_fence_before_sync();
   __syncthreads();  // P is written, the state's part has been read
   if (warp == 0) {
     if (elect_one() && !*abort_flag) {
       tc_fence_after_sync();
-      const uint64_t dC = mdesc(smem_u32(sC));
+      const uint64_t dV = mdesc(smem_u32(sV));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(tAcc, tP + 8 * k, dC + 128 * k, kIdescC, k > 0);
+      for (int k = 0; k < 8; ++k) mma_ts(tAcc, tP + 8 * k, dV + 128 * k, kIdescAcc, k > 0);
       mma_commit(&bar_mma[2]);
     }
     __syncwarp();
   }
   wait_bar_warp(&bar_mma[2], 0, abort_flag, kWaitChunkMma, chunk);
   tc_fence_after_sync();
-  float dot = 0.f, across = 0.f;
-  {
-    uint32_t r[32];
-    tmem_ld_x32(tAcc + lane_base + 32 * hf, r);
-    tmem_ld_wait();
-    if constexpr (PASS == kGsDk) across = with_state ? dot_of(acc) : 0.f;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) acc[j] += __uint_as_float(r[j]);
-  }
-  if constexpr (MT) {
-    dot = dot_of(acc) - across;
-    if (hf) sDot[0][row] = dot, sDot[1][row] = across;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 u;
-    u.x = Pack2<T>::pack(acc[8 * j], acc[8 * j + 1]), u.y = Pack2<T>::pack(acc[8 * j + 2], acc[8 * j + 3]);
-    u.z = Pack2<T>::pack(acc[8 * j + 4], acc[8 * j + 5]), u.w = Pack2<T>::pack(acc[8 * j + 6], acc[8 * j + 7]);
-    *tile_piece(sC, row, 4 * hf + j) = u;  // (the MMAs that read C have completed)
-  }
+  acc_add(acc, tAcc + lane_base + 32 * hf);
+  stage_row<T>(sV, row, 4 * hf, acc);  // (the MMAs that read V have completed)
   fence_proxy_async_smem();
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 0) {
     if (elect_one()) {
       if (!*abort_flag) {
-        tma_store_tile_x(&mapO, sC, 64 * J, c0, h, static_cast<int>(b));
+        tma_store_tile_x(&mapO, sV, 64 * J, c0, h, static_cast<int>(b));
         tma_store_commit();
         tma_store_wait_read<0>();
       } else {
@@ -636,57 +631,213 @@ __device__ __forceinline__ void gated_chunk_tc(const CUtensorMap& mapA, const CU
   } else if (warp == 1) {
     tmem_dealloc(tP, 128);
   }
-  if constexpr (MT) {
-    if (!hf) {
-      const long o = (J * a.units + unit) * kGtChunk + row;
-      (PASS == kGsDq ? a.qdot : a.kdot)[o] = dot + sDot[0][row];
-      if (PASS == kGsDk) a.bdot[o] = across + sDot[1][row];
-    }
-  }
 }
 
-// FWD: grid = B*H * chunks * D/64.  Backward: three times as many; the CTAs of a chunk are neighbours, so that its tiles are read
-// from memory once and from L2 after that.
-template <typename T, int D, bool FWD>
-__global__ void __launch_bounds__(kGtThreads, D == 64 ? 3 : 2) gated_chunk_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a) {
-  constexpr int NT = D / 64;
-  const long t = blockIdx.x;
-  if constexpr (FWD) {
-    gated_chunk_tc<T, D, kGsOut>(m.q, m.k, m.v, m.o, a, t / NT, static_cast<int>(t % NT));
-  } else {
-    const long unit = t / (3 * NT);
-    const int r = static_cast<int>(t % (3 * NT)), J = r % NT;
-    if (r / NT == 0)
-      gated_chunk_tc<T, D, kGsDq>(m.o, m.v, m.k, m.dq, a, unit, J);
-    else if (r / NT == 1)
-      gated_chunk_tc<T, D, kGsDk>(m.v, m.o, m.q, m.dk, a, unit, J);
-    else
-      gated_chunk_tc<T, D, kGsDv>(m.k, m.q, m.o, m.dv, a, unit, J);
-  }
-}
+struct GatedMaps {
+  CUtensorMap q, k, v, o, dq, dk, dv;
+};
+template <int D> constexpr int bwd_threads() { return 4 * D; }
+template <int D> constexpr size_t bwd_tc_smem() { return 1024 + 4 * (D / 64) * kTileBytes + 2 * (D / 64) * (D / 64) * kStateTile; }
 
-// dg of a chunk.  With k.dk split into what the chunk itself contributes and what lies across its end,
+// Backward of one chunk: dq, dk, dv and dg from q, k, v, dO and the two states, each read once; grid = B*H * chunks.
+//     E  = dO V^T  (t, s)    dq = e^(G_t) dO S^T        + (E D) K
+//     E' = V dO^T  (s, t)    dk = e^(G_last-G_s) V R^T  + (E' D) Q
+//     P' = K Q^T   (s, t)    dv = e^(G_last-G_s) K R    + (P' D) dO
+// E and its transpose are both computed: an A operand from TMEM cannot be transposed, and two products of 128 x 128 x D cost less
+// than a 32 KB tile through shared memory.  Two score buffers X and Y in TMEM; every pass is scores -> decayed 16-bit scores in
+// place -> the state's part into the accumulator (D 64: the buffer's other half), read and scaled in fp32 -> scores times rows.  The
+// passes are interleaved so that the MMAs of one run under the register work of another:
+//     E X, E' Y | decay X | state X | decay Y | state Y | rows X | rows Y | dq out, P' X | decay X, dk out | state X | rows X | dv out
+// Results are staged over the tile that has no reader left: dq over V, dk over Q, dv over K.
+// With k.dk split into what the chunk itself contributes and what lies across its end,
 //     dg_t = sum_{u>=t} (q_u.dq_u - (k_u.dk_u)_within) + sum_{s<t} (k_s.dk_s)_across + A <S, R>
 // counts the pairs that cross t and no others, but for those within the chunk, which are the same rounded products in q.dq and in
 // k.dk and cancel.  (gated_simt.cuh has <S', R> for the last two terms; with operands of 16 bits that would leave the roundings of all
-// pairs across the chunk's end at every position.)  The two states are the tiles that the products used, whose layouts are alike.
-// grid = B*H * chunks, block = 128.
+// pairs across the chunk's end at every position.)
+//   warp w: rows 32 (w % 4) .., group w / 4 of D / 32: 4096 / D columns of the scores and 32 of the accumulator
 template <typename T, int D>
-__global__ void __launch_bounds__(kGtChunk) gated_dgate_tc_kernel(const GatedChunkArgs a, void* dgate, const cott_strides sdg) {
-  constexpr int NT = D / 64;
-  __shared__ float part[16];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(bwd_threads<D>(), D == 64 ? 2 : 1)
+gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a) {
+  using namespace ptx;
+  constexpr int NT = D / 64, NG = D / 32, NB = 4 / NG;  // column groups; 32-column blocks of the scores per warp
+  constexpr uint32_t kCols = D == 64 ? 256 : 512, kBuf = kCols / 2, kAccAt = D == 64 ? 64 : 128;
+  constexpr bool BF = Pack2<T>::kBf16;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char *sQ = smem, *sK = sQ + NT * kTileBytes, *sV = sK + NT * kTileBytes, *sO = sV + NT * kTileBytes, *sS = sO + NT * kTileBytes,
+                *sR = sS + NT * NT * kStateTile;
+  __shared__ uint64_t bar_full, bar_score[3], bar_state[3], bar_rows[3];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag_s;
+  __shared__ __align__(16) float sG[kGtChunk], sLow[4][kGtChunk], sUp[4][kGtChunk];
+  __shared__ float sQd[NG][kGtChunk], sKd[NG][kGtChunk], sBd[NG][kGtChunk], sCross[4 * NG], sPart[8];
+  volatile int* abort_flag = &abort_flag_s;
+
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int wq = warp & 3, cg = warp >> 2, row = 32 * wq + lane;
   const long unit = blockIdx.x, bh = unit / a.nchunks, b = bh / a.H;
-  const int chunk = static_cast<int>(unit % a.nchunks), h = static_cast<int>(bh % a.H), pos = chunk * kGtChunk + tid;
+  const int chunk = static_cast<int>(unit % a.nchunks), h = static_cast<int>(bh % a.H), c0 = chunk * kGtChunk, bi = static_cast<int>(b);
+  const bool with_S = chunk > 0 || a.with_first, with_R = chunk + 1 < a.nchunks || a.with_last;
+  const uint32_t lane_base = static_cast<uint32_t>(32 * wq) << 16;
+  if (tid == 0) {
+    mbar_init(&bar_full, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&bar_score[i], 1);
+      mbar_init(&bar_state[i], 1);
+      mbar_init(&bar_rows[i], 1);
+    }
+    mbar_fence_init();
+    abort_flag_s = 0;
+    tma_prefetch_desc(&m.q);
+    tma_prefetch_desc(&m.k);
+    tma_prefetch_desc(&m.v);
+    tma_prefetch_desc(&m.o);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
   pdl_allow_next();
   pdl_wait_prior();
-  const float g = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, pos);
+  const uint32_t tX = tmem_slot, tY = tX + kBuf;
+  if (warp == 0) {
+    if (elect_one()) {
+      mbar_expect_tx(&bar_full, 4 * NT * kTileBytes + ((with_S ? 1 : 0) + (with_R ? 1 : 0)) * NT * NT * kStateTile);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        tma_load_tile_x(sO + i * kTileBytes, &m.o, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sV + i * kTileBytes, &m.v, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sK + i * kTileBytes, &m.k, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sQ + i * kTileBytes, &m.q, &bar_full, 64 * i, c0, h, bi);
+      }
+      if (with_S) bulk_load(sS, a.S + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
+      if (with_R) bulk_load(sR, a.R + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
+    }
+    __syncwarp();
+  } else if (warp == 4) {
+    chunk_gates<T>(a, sG, b, h, c0, lane);
+  }
+  const bool kp = !a.keep || (c0 + row < a.N && a.keep[b * a.N + c0 + row]);
+  __syncthreads();
+  for (int e = tid; e < 4 * kGtChunk; e += bwd_threads<D>()) {
+    col_factor<true>(sLow, sG, e >> 7, e & 127);
+    col_factor<false>(sUp, sG, e >> 7, e & 127);
+  }
+  // (every thread reads rows of the tiles later on, so every thread waits for them)
+  wait_bar_warp(&bar_full, 0, abort_flag, kWaitChunkTma, chunk);
+  if (a.keep) {  // nothing of a masked position gets into a product
+    if (!kp) {
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 8; ++j)
+        for (int i = cg; i < 4 * NT; i += NG) *tile_piece(sQ + i * kTileBytes, row, j) = zero;
+    }
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, D, BF, false, false), kIdescM = make_idesc(128, D, BF, false, true);
+  constexpr uint64_t kPanel = kTileBytes >> 4, kStatePanel = (NT * kStateTile) >> 4;
+  const uint64_t dQ = kdesc(smem_u32(sQ)), dK = kdesc(smem_u32(sK)), dV = kdesc(smem_u32(sV)), dO = kdesc(smem_u32(sO));
+  auto scores = [&](uint32_t t, uint64_t dA, uint64_t dB, uint64_t* bar) {  // t = A B^T
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k) mma_ss(t, dA + (k >> 2) * kPanel + 2 * (k & 3), dB + (k >> 2) * kPanel + 2 * (k & 3), kIdescP, k > 0);
+    mma_commit(bar);
+  };
+  auto times_rows = [&](uint32_t t, unsigned char* tile, uint64_t* bar) {  // acc = (scores in TMEM) rows
+    const uint64_t d = make_smem_desc(smem_u32(tile), kTileBytes, 1024);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mma_ts(t + kAccAt, t + 8 * k, d + 128 * k, kIdescM, k > 0);
+    mma_commit(bar);
+  };
+  auto times_state_t = [&](uint32_t t, uint64_t dA, unsigned char* state, uint64_t* bar) {  // acc = A M^T
+    const uint64_t d = kdesc(smem_u32(state));
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k) mma_ss(t + kAccAt, dA + (k >> 2) * kPanel + 2 * (k & 3), d + (k >> 2) * kStatePanel + 2 * (k & 3), kIdescK, k > 0);
+    mma_commit(bar);
+  };
+  auto times_state = [&](uint32_t t, uint64_t dA, unsigned char* state, uint64_t* bar) {  // acc = A M
+    const uint64_t d = make_smem_desc(smem_u32(state), NT * kStateTile, 1024);
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k) mma_ss(t + kAccAt, dA + (k >> 2) * kPanel + 2 * (k & 3), d + 128 * k, kIdescM, k > 0);
+    mma_commit(bar);
+  };
+  // `body` by one thread (chosen by elect.sync where it issues: see elect_one), if nothing has given up; after the barrier that
+  // everybody's TMEM accesses came before
+  auto issue = [&](bool cond, auto&& body) {
+    if (warp == 0) {
+      if (elect_one() && cond && !*abort_flag) {
+        tc_fence_after_sync();
+        body();
+      }
+      __syncwarp();
+    }
+  };
+  auto sync = [&]() {
+    tc_fence_before_sync();
+    __syncthreads();
+  };
+  auto wait = [&](uint64_t* bar) {
+    wait_bar_warp(bar, 0, abort_flag, kWaitChunkMma, chunk);
+    tc_fence_after_sync();
+  };
+  const uint32_t my_scores = lane_base, my_acc = lane_base + kAccAt + 32 * cg;
+  auto put_scores = [&](uint32_t t, const uint32_t (&pk)[NB][16]) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) tmem_st_x16(t + lane_base + 16 * (NB * cg + i), pk[i]);
+    tmem_st_wait();
+  };
+  issue(true, [&] {
+    scores(tX, dO, dV, &bar_score[0]);
+    scores(tY, dV, dO, &bar_score[1]);
+  });
+  const float Gr = sG[row], total = sG[kGtChunk - 1];
+  const float head = __expf(Gr), tail = __expf(total - Gr);
+  const float row_low = __expf(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = __expf(sG[32 * wq + 31] - Gr);
+  const int panel = cg / 2 * kTileBytes, j0 = 4 * (cg & 1);  // where this thread's 32 columns are in a row of D
+
+  uint32_t pk[NB][16];
+  float ax[32], ay[32];
+  // ---- dq: decayed scores X
+  wait(&bar_score[0]);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) decay_block<T, true>(pk[i], tX + my_scores, NB * cg + i, wq, lane, Gr, row_low, sG, sLow[wq]);
+  sync();
+  issue(with_S, [&] { times_state_t(tX, dO, sS, &bar_state[0]); });
+  put_scores(tX, pk);
+  // ---- dk: decayed scores Y
+  wait(&bar_score[1]);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) decay_block<T, false>(pk[i], tY + my_scores, NB * cg + i, wq, lane, Gr, row_up, sG, sUp[wq]);
+  sync();
+  issue(with_R, [&] { times_state_t(tY, dV, sR, &bar_state[1]); });
+  put_scores(tY, pk);
+  // ---- dq: the state's part, then the rows
+#pragma unroll
+  for (int j = 0; j < 32; ++j) ax[j] = 0.f, ay[j] = 0.f;
+  if (with_S) {
+    wait(&bar_state[0]);
+    acc_scaled(ax, tX + my_acc, head);
+  }
+  sync();
+  issue(true, [&] { times_rows(tX, sK, &bar_rows[0]); });
+  // ---- dk: the same
+  if (with_R) {
+    wait(&bar_state[1]);
+    acc_scaled(ay, tY + my_acc, tail);
+  }
+  sync();
+  issue(true, [&] { times_rows(tY, sQ, &bar_rows[1]); });
+  // ---- <S, R>, and what of k.dk lies across the chunk's end
+  sBd[cg][row] = with_R ? row_dot32<T>(sK + panel, row, j0, ay) : 0.f;
   float cross = 0.f;
-  if ((chunk > 0 || a.with_first) && (chunk + 1 < a.nchunks || a.with_last)) {
-    const uint4 *S = reinterpret_cast<const uint4*>(a.S + unit * (NT * NT * kStateTile)), *R = reinterpret_cast<const uint4*>(a.R + unit * (NT * NT * kStateTile));
-#pragma unroll 4
-    for (int e = tid; e < NT * NT * kStateTile / 16; e += kGtChunk) {
-      const uint4 x = S[e], y = R[e];
+  if (with_S && with_R) {
+    const uint4 *s4 = reinterpret_cast<const uint4*>(sS), *r4 = reinterpret_cast<const uint4*>(sR);
+#pragma unroll 2
+    for (int e = tid; e < NT * NT * kStateTile / 16; e += bwd_threads<D>()) {
+      const uint4 x = s4[e], y = r4[e];
       const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -694,42 +845,103 @@ __global__ void __launch_bounds__(kGtChunk) gated_dgate_tc_kernel(const GatedChu
         cross = fmaf(f.x, f2.x, fmaf(f.y, f2.y, cross));
       }
     }
-  }
-  float d = 0.f, across = 0.f;
 #pragma unroll
-  for (int J = 0; J < NT; ++J) {
-    const long o = (J * a.units + unit) * kGtChunk + tid;
-    d += a.qdot[o] - a.kdot[o];
-    across += a.bdot[o];
+    for (int off = 16; off > 0; off >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, off);
   }
-  float total = g, run = d, up = across;  // of the warp: the gates' sum, d from the row to the warp's end, across up to the row
+  if (lane == 0) sCross[warp] = cross;
+  // ---- dq out, P' into X
+  wait(&bar_rows[0]);
+  acc_add(ax, tX + my_acc);
+  sQd[cg][row] = row_dot32<T>(sQ + panel, row, j0, ax);
+  stage_row<T>(sV + panel, row, j0, ax);  // (V's readers: the scores and dk's state part, all complete)
+  fence_proxy_async_smem();
+  sync();
+  issue(true, [&] {
+    scores(tX, dK, dQ, &bar_score[2]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    cross += __shfl_xor_sync(0xffffffffu, cross, off);
-    total += __shfl_xor_sync(0xffffffffu, total, off);
-  }
+    for (int i = 0; i < NT; ++i) tma_store_tile_x(&m.dq, sV + i * kTileBytes, 64 * i, c0, h, bi);
+    tma_store_commit();
+  });
+  // ---- dv: decayed scores X
+  wait(&bar_score[2]);
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const float x = __shfl_down_sync(0xffffffffu, run, off), y = __shfl_up_sync(0xffffffffu, up, off);
-    if (lane + off < 32) run += x;
-    if (lane >= off) up += y;
+  for (int i = 0; i < NB; ++i) decay_block<T, false>(pk[i], tX + my_scores, NB * cg + i, wq, lane, Gr, row_up, sG, sUp[wq]);
+  sync();
+  issue(with_R, [&] { times_state(tX, dK, sR, &bar_state[2]); });
+  put_scores(tX, pk);
+  // ---- dk out
+  wait(&bar_rows[1]);
+  {
+    float y[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = 0.f;
+    acc_add(y, tY + my_acc);
+    sKd[cg][row] = row_dot32<T>(sK + panel, row, j0, y);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) ay[j] += y[j];
   }
-  if (lane == 0) part[warp] = cross, part[4 + warp] = run, part[12 + warp] = total;
-  if (lane == 31) part[8 + warp] = up;
-  __syncthreads();
-  float before = __shfl_up_sync(0xffffffffu, up, 1);
-  if (lane == 0) before = 0.f;
-  const float A = __expf((part[12] + part[13]) + (part[14] + part[15]));
-  float x = run + before + (A == 0.f ? 0.f : A * ((part[0] + part[1]) + (part[2] + part[3])));
-  for (int w = 0; w < 4; ++w) x += w > warp ? part[4 + w] : w < warp ? part[8 + w] : 0.f;
-  if (pos < a.N) {
-    if ((a.keep && !a.keep[b * a.N + pos]) || (pos == 0 && !a.with_first) || g <= kGateFloorTc) x = 0.f;
-    const long long o = b * sdg.b + h * sdg.h + static_cast<long long>(pos) * sdg.n;
+  stage_row<T>(sQ + panel, row, j0, ay);  // (Q's readers: dk's rows and P', both complete)
+  fence_proxy_async_smem();
+  // ---- dv: the state's part, then the rows
+#pragma unroll
+  for (int j = 0; j < 32; ++j) ax[j] = 0.f;
+  if (with_R) {
+    wait(&bar_state[2]);
+    acc_scaled(ax, tX + my_acc, tail);
+  }
+  sync();
+  issue(true, [&] {
+    times_rows(tX, sO, &bar_rows[2]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) tma_store_tile_x(&m.dk, sQ + i * kTileBytes, 64 * i, c0, h, bi);
+    tma_store_commit();
+  });
+  // ---- dg (the first four warps: a position each)
+  float x = 0.f;
+  if (warp < 4) {
+    float run = 0.f, up = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) run += sQd[i][row] - sKd[i][row], up += sBd[i][row];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {  // run: from the row to the warp's end; up: to the row
+      const float d = __shfl_down_sync(0xffffffffu, run, off), u = __shfl_up_sync(0xffffffffu, up, off);
+      if (lane + off < 32) run += d;
+      if (lane >= off) up += u;
+    }
+    if (lane == 0) sPart[warp] = run;
+    if (lane == 31) sPart[4 + warp] = up;
+    const float before = __shfl_up_sync(0xffffffffu, up, 1);
+    x = run + (lane ? before : 0.f);
+  }
+  // ---- dv out
+  wait(&bar_rows[2]);
+  acc_add(ax, tX + my_acc);
+  stage_row<T>(sK + panel, row, j0, ax);  // (K's readers: dq's rows, P' and dv's state part, all complete)
+  fence_proxy_async_smem();
+  sync();
+  issue(true, [&] {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) tma_store_tile_x(&m.dv, sK + i * kTileBytes, 64 * i, c0, h, bi);
+    tma_store_commit();
+  });
+  if (tid == 0 && *abort_flag) mbar_wait(&bar_full, 0, 64);  // no load may be in flight when the CTA leaves
+  if (warp == 1) tmem_dealloc(tX, kCols);
+  if (warp < 4 && c0 + row < a.N && !*abort_flag) {
+    float sr = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4 * NG; ++i) sr += sCross[i];
+    const float A = __expf(total);
+    x += A == 0.f ? 0.f : A * sr;
+    for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
+    const int pos = c0 + row;
+    if (!kp || (pos == 0 && !a.with_first) || gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, pos) <= kGateFloorTc) x = 0.f;
+    const long long o = b * a.sdg.b + h * a.sdg.h + static_cast<long long>(pos) * a.sdg.n;
     if (a.gate_f32)
-      static_cast<float*>(dgate)[o] = x;
+      static_cast<float*>(a.dgate)[o] = x;
     else
-      static_cast<T*>(dgate)[o] = from_acc<T>(x);
+      static_cast<T*>(a.dgate)[o] = from_acc<T>(x);
   }
+  issue(true, [&] { tma_store_wait_read<0>(); });
 }
 
 }  // namespace cott

@@ -76,35 +76,32 @@ GatedTcArgs walk_args(const GatedArgs& g) {
 }
 GatedChunkArgs chunk_args(const GatedArgs& g, long bh) {
   GatedChunkArgs c = {};
-  c.gate = g.gate, c.keep = g.keep, c.sg = g.sg, c.H = g.H, c.N = g.N, c.nchunks = tc_chunks(g.N), c.gate_f32 = g.gate_f32;
+  c.gate = g.gate, c.keep = g.keep, c.sg = g.sg, c.sdg = g.sdg, c.H = g.H, c.N = g.N, c.nchunks = tc_chunks(g.N), c.gate_f32 = g.gate_f32;
   c.units = bh * c.nchunks, c.with_first = g.with_initial;
   return c;
 }
 
 template <typename T, int D>
 int run_tc_fwd(const GatedArgs& g, void* states, void* ws, int B, int dtype, cudaStream_t stream) {
-  constexpr int NT = D / 64;
   const long bh = (long)B * g.H;
-  GatedMaps m;
-  TRY(make_map(&m.q, g.q, g.sq, B, g.H, g.N, D, dtype));
-  TRY(make_map(&m.k, g.k, g.sk, B, g.H, g.N, D, dtype));
-  TRY(make_map(&m.v, g.v, g.sv, B, g.H, g.N, D, dtype));
-  TRY(make_map(&m.o, g.out, g.so, B, g.H, g.N, D, dtype));
-  m.dq = m.dk = m.dv = m.o;
+  CUtensorMap q, k, v, o;
+  TRY(make_map(&q, g.q, g.sq, B, g.H, g.N, D, dtype));
+  TRY(make_map(&k, g.k, g.sk, B, g.H, g.N, D, dtype));
+  TRY(make_map(&v, g.v, g.sv, B, g.H, g.N, D, dtype));
+  TRY(make_map(&o, g.out, g.so, B, g.H, g.N, D, dtype));
   GatedTcArgs a = walk_args(g);
   a.edge = g.initial, a.last = g.final_state, a.states = static_cast<unsigned char*>(states);
-  TRY((launch_walk<T, D, false>(a, m.k, m.v, bh, ws, stream)));
+  TRY((launch_walk<T, D, false>(a, k, v, bh, ws, stream)));
   GatedChunkArgs c = chunk_args(g, bh);
   c.S = a.states;
-  auto kern = gated_chunk_tc_kernel<T, D, true>;
-  COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_tc_smem<D>()));
-  COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(c.units * NT)), kGtThreads, chunk_tc_smem<D>(), stream, m, c));
+  auto kern = gated_fwd_tc_kernel<T, D>;
+  COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fwd_tc_smem<D>()));
+  COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(c.units * (D / 64))), kFwdThreads, fwd_tc_smem<D>(), stream, q, k, v, o, c));
   return COTT_OK;
 }
 
 template <typename T, int D>
 int run_tc_bwd(const GatedArgs& g, const void* states, void* ws, int B, int dtype, cudaStream_t stream) {
-  constexpr int NT = D / 64;
   const long bh = (long)B * g.H;
   GatedMaps m;
   TRY(make_map(&m.q, g.q, g.sq, B, g.H, g.N, D, dtype));
@@ -118,15 +115,11 @@ int run_tc_bwd(const GatedArgs& g, const void* states, void* ws, int B, int dtyp
   unsigned char* p = static_cast<unsigned char*>(ws);
   a.edge = g.dfinal, a.last = g.dinitial, a.states = p;
   GatedChunkArgs c = chunk_args(g, bh);
-  p += round256(c.units * tile_bytes(D));
-  c.qdot = reinterpret_cast<float*>(p), c.kdot = c.qdot + NT * c.units * kGtChunk, c.bdot = c.kdot + NT * c.units * kGtChunk;
-  p += round256(3 * NT * c.units * kGtChunk * sizeof(float));
-  TRY((launch_walk<T, D, true>(a, m.q, m.o, bh, p, stream)));
-  c.S = static_cast<const unsigned char*>(states), c.R = a.states, c.q = g.q, c.k = g.k, c.sq = g.sq, c.sk = g.sk, c.with_last = g.dfinal != nullptr;
-  auto kern = gated_chunk_tc_kernel<T, D, false>;
-  COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_tc_smem<D>()));
-  COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(c.units * 3 * NT)), kGtThreads, chunk_tc_smem<D>(), stream, m, c));
-  COTT_CUDA_TRY(launch_pdl(gated_dgate_tc_kernel<T, D>, dim3((unsigned)c.units), kGtChunk, 0, stream, c, g.dgate, g.sdg));
+  TRY((launch_walk<T, D, true>(a, m.q, m.o, bh, p + round256(c.units * tile_bytes(D)), stream)));
+  c.S = static_cast<const unsigned char*>(states), c.R = a.states, c.dgate = g.dgate, c.with_last = g.dfinal != nullptr;
+  auto kern = gated_bwd_tc_kernel<T, D>;
+  COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd_tc_smem<D>()));
+  COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)c.units), bwd_threads<D>(), bwd_tc_smem<D>(), stream, m, c));
   return COTT_OK;
 }
 
@@ -142,7 +135,7 @@ size_t gated_tc_workspace_bytes(int B, int H, int N, int D, bool backward) {
   const long bh = (long)B * H;
   if (!backward) return seg_bytes(bh, N, D);
   const size_t units = (size_t)bh * tc_chunks(N);
-  return round256(units * tile_bytes(D)) + round256(3 * (D / 64) * units * kGtChunk * sizeof(float)) + seg_bytes(bh, N, D);
+  return round256(units * tile_bytes(D)) + seg_bytes(bh, N, D);
 }
 
 int gated_tc_fwd(const GatedArgs& g, void* states, void* workspace, int B, int D, int dtype, cudaStream_t stream) {

@@ -88,7 +88,13 @@ def test_gates_of_one_strength(dtype, level):
         # dg is e^level of the terms that it is summed from: a position's own pair, (q_t.k_t)(dO_t.v_t), stands in q_t.dq_t and in
         # k_t.dk_t and cancels.  Those terms are products |q| |dq| of about 1 x 8, each with a rounding of 2^-24 (16 bits: u, of the
         # same rounded product in both, so that fp32's remains, and the state's), and up to 64 (128) of either kind are summed.
-        _compare((*got[:5], *got[6:]), (*want[:5], *want[6:]), dtype)
+        if dtype == torch.float16 and level == -30.0:
+            # the gradient of the initial state is e^-30 of its terms: products below the type's smallest step, 2^-24, which the
+            # weighted rows are rounded to in absolute terms (half of it, times the sum of |q| <= 128 over a chunk)
+            assert (got[6].double().cpu() - want[6]).abs().max() <= 2 ** -25 * 128
+            _compare(got[:5], want[:5], dtype)
+        else:
+            _compare((*got[:5], *got[6:]), (*want[:5], *want[6:]), dtype)
         rms = (got[5].double().cpu() - want[5]).square().mean().sqrt()
         assert rms <= 8 * 2 ** -24 * 256 ** 0.5 + (0 if dtype == torch.float32 else _u(dtype) * want[5].square().mean().sqrt() * 6 + 1e-4 * _u(dtype) / _u(torch.bfloat16))
     else:
