@@ -944,4 +944,382 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
   issue(true, [&] { tma_store_wait_read<0>(); });
 }
 
+// ---- backward at head dim 64: a persistent kernel ------------------------------------------------------------------------
+// The same three passes, a group of four warps for each, side by side.  A thread owns a row, so that scores are decayed and packed
+// in place without a word to the other warps, and everything a group does per chunk is a handful of rolled loops that all three run
+// (the one-chunk kernel spent a quarter of its time waiting for instructions and another at its barriers):
+//     scores (MMA) -> decay, pack -> state's part (MMA) -> scale -> rows (MMA) -> result over a tile -> TMA
+//   warps 0-3: dq over Q     4-7: dk over K     8-11: dv over V     (rows and TMEM lanes 32 (w % 4) ..)
+//   warps 12-15: gates of the next chunk, masked rows, <S, R>, dg   warp 16: TMA loads
+// Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group: scores, then the packed scores and the accumulator.
+// A result is staged over a tile when the MMAs that read it have completed, whichever group issued them; the barriers for that are
+// kept per stage, so that nobody can be a whole phase ahead of one that is still waiting.
+// Every wait is bounded.  After one that gave up, nothing more is issued, every further wait returns at once and all warps still go
+// through all named barriers.
+constexpr int kBwd64Threads = 544;
+constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
+constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
+
+struct __align__(16) BwdInfo {  // of a stage's chunk
+  float G[kGtChunk], low[4][kGtChunk], up[4][kGtChunk];
+  float gate[kGtChunk], qd[kGtChunk], kd[kGtChunk], bd[kGtChunk];
+};
+
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+template <typename T>
+__global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a) {
+  using namespace ptx;
+  constexpr bool BF = Pack2<T>::kBf16;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ BwdInfo info[2];
+  __shared__ uint64_t bar_full[2], bar_free[2], bar_ready[2], bar_dots[2], bar_score[3][2], bar_state[3][2], bar_rows[3][2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ float sPart[12];
+  __shared__ int abort_flag_s, loads_s;
+  volatile int* abort_flag = &abort_flag_s;
+
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int wq = warp & 3, row = 32 * wq + lane;
+  const uint32_t lane_base = static_cast<uint32_t>(32 * wq) << 16;
+  auto tile_o = [&](int s) { return smem + s * kBwd64Stage; };
+  auto tile_v = [&](int s) { return smem + s * kBwd64Stage + kTileBytes; };
+  auto tile_k = [&](int s) { return smem + s * kBwd64Stage + 2 * kTileBytes; };
+  auto tile_q = [&](int s) { return smem + s * kBwd64Stage + 3 * kTileBytes; };
+  auto state_s = [&](int s) { return smem + s * kBwd64Stage + 4 * kTileBytes; };
+  auto state_r = [&](int s) { return smem + s * kBwd64Stage + 4 * kTileBytes + kStateTile; };
+  auto has_s = [&](int chunk) { return chunk > 0 || a.with_first; };
+  auto has_r = [&](int chunk) { return chunk + 1 < a.nchunks || a.with_last; };
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar_full[s], 1);
+      mbar_init(&bar_free[s], 7);   // three stores, four warps that took <S, R>
+      mbar_init(&bar_ready[s], 4);
+      mbar_init(&bar_dots[s], 8);
+      for (int p = 0; p < 3; ++p) {
+        mbar_init(&bar_score[p][s], 1);
+        mbar_init(&bar_state[p][s], 1);
+        mbar_init(&bar_rows[p][s], 1);
+      }
+    }
+    mbar_fence_init();
+    abort_flag_s = 0;
+    loads_s = 0;
+    tma_prefetch_desc(&m.q);
+    tma_prefetch_desc(&m.k);
+    tma_prefetch_desc(&m.v);
+    tma_prefetch_desc(&m.o);
+  }
+  if (warp == 16) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  pdl_allow_next();
+  pdl_wait_prior();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 16) {
+    // ---------------------------------------------------------------- loads
+    if (elect_one()) {
+      int n = 0;
+      for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
+        const int s = n & 1;
+        if (n >= 2 && !wait_bar(&bar_free[s], ((n >> 1) - 1) & 1, abort_flag, kWaitWalkFree, n)) break;
+        const long bh = unit / a.nchunks;
+        const int chunk = static_cast<int>(unit % a.nchunks), h = static_cast<int>(bh % a.H), b = static_cast<int>(bh / a.H), c0 = chunk * kGtChunk;
+        mbar_expect_tx(&bar_full[s], 4 * kTileBytes + ((has_s(chunk) ? 1 : 0) + (has_r(chunk) ? 1 : 0)) * kStateTile);
+        tma_load_tile(tile_o(s), &m.o, &bar_full[s], c0, h, b);
+        tma_load_tile(tile_v(s), &m.v, &bar_full[s], c0, h, b);
+        tma_load_tile(tile_k(s), &m.k, &bar_full[s], c0, h, b);
+        tma_load_tile(tile_q(s), &m.q, &bar_full[s], c0, h, b);
+        if (has_s(chunk)) bulk_load(state_s(s), a.S + unit * kStateTile, kStateTile, &bar_full[s]);
+        if (has_r(chunk)) bulk_load(state_r(s), a.R + unit * kStateTile, kStateTile, &bar_full[s]);
+        loads_s = n + 1;
+      }
+    }
+  } else if (warp >= 12) {
+    // ---------------------------------------------------------------- gates, masked rows, <S, R>, dg
+    const int t = tid - 384;  // position
+    float g[4], gt = 0.f, cross_before = 0.f;
+    bool kp = true, kp_before = true;
+    auto fetch = [&](long unit) {
+      const long bh = unit / a.nchunks, b = bh / a.H;
+      const int c0 = static_cast<int>(unit % a.nchunks) * kGtChunk, h = static_cast<int>(bh % a.H);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
+      gt = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + t);
+      kp = !a.keep || (c0 + t < a.N && a.keep[b * a.N + c0 + t]);
+    };
+    // dg of the chunk before (unit u, the n-th of this CTA): its dot products, <S, R> as this warp's part
+    auto write_dgate = [&](long u, int n, float cross, bool kept) {
+      const BwdInfo& f = info[n & 1];
+      wait_bar_warp(&bar_dots[n & 1], (n >> 1) & 1, abort_flag, kWaitAcc, n);
+      const long bh = u / a.nchunks, b = bh / a.H;
+      const int chunk = static_cast<int>(u % a.nchunks), h = static_cast<int>(bh % a.H), pos = chunk * kGtChunk + t;
+      float run = f.qd[t] - f.kd[t], up = f.bd[t];
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {  // run: from the row to the warp's end; up: to the row
+        const float d = __shfl_down_sync(0xffffffffu, run, off), x = __shfl_up_sync(0xffffffffu, up, off);
+        if (lane + off < 32) run += d;
+        if (lane >= off) up += x;
+      }
+      named_sync(4, 128);  // (the sums of the chunk before have been read)
+      if (lane == 0) sPart[wq] = run, sPart[8 + wq] = cross;
+      if (lane == 31) sPart[4 + wq] = up;
+      const float before = __shfl_up_sync(0xffffffffu, up, 1);
+      named_sync(4, 128);
+      const float A = __expf(f.G[kGtChunk - 1]);
+      float x = run + (lane ? before : 0.f) + (A == 0.f ? 0.f : A * ((sPart[8] + sPart[9]) + (sPart[10] + sPart[11])));
+      for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
+      if (pos < a.N && !*abort_flag) {
+        if (!kept || (pos == 0 && !a.with_first) || f.gate[t] <= kGateFloorTc) x = 0.f;
+        const long long o = b * a.sdg.b + h * a.sdg.h + static_cast<long long>(pos) * a.sdg.n;
+        if (a.gate_f32)
+          static_cast<float*>(a.dgate)[o] = x;
+        else
+          static_cast<T*>(a.dgate)[o] = from_acc<T>(x);
+      }
+    };
+    int n = 0;
+    long unit = blockIdx.x;
+    if (unit < a.units) fetch(unit);
+    for (; unit < a.units; unit += gridDim.x, ++n) {
+      const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
+      const bool kept = kp;
+      const float gate = gt;
+      gate_sums<false>(g, lane);
+      wait_bar_warp(&bar_full[s], (n >> 1) & 1, abort_flag, kWaitChunkTma, n);  // (and nobody uses the stage's tables any more)
+      BwdInfo& f = info[s];
+      if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
+      f.gate[t] = gate;
+      if (unit + gridDim.x < a.units) fetch(unit + gridDim.x);
+      named_sync(4, 128);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        col_factor<true>(f.low, f.G, w, t);
+        col_factor<false>(f.up, f.G, w, t);
+      }
+      if (a.keep) {  // nothing of a masked position gets into a product
+        if (!kept) {
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 8; ++j)
+            for (int i = 0; i < 4; ++i) *tile_piece(tile_o(s) + i * kTileBytes, t, j) = zero;
+        }
+        fence_proxy_async_smem();
+      }
+      warp_arrive(&bar_ready[s], lane);
+      float cross = 0.f;
+      if (has_s(chunk) && has_r(chunk)) {
+        const uint4 *x4 = reinterpret_cast<const uint4*>(state_s(s)), *y4 = reinterpret_cast<const uint4*>(state_r(s));
+#pragma unroll
+        for (int e = 0; e < kStateTile / 16 / 128; ++e) {
+          const uint4 x = x4[t + 128 * e], y = y4[t + 128 * e];
+          const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p = Pack2<T>::unpack(u[i]), q = Pack2<T>::unpack(w[i]);
+            cross = fmaf(p.x, q.x, fmaf(p.y, q.y, cross));
+          }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, off);
+      }
+      warp_arrive(&bar_free[s], lane);
+      if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
+      cross_before = cross;
+      kp_before = kept;
+    }
+    if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
+  } else {
+    // ---------------------------------------------------------------- the passes
+    const int pass = warp >> 2;  // 0 dq, 1 dk, 2 dv
+    const bool lower = pass == 0;
+    const uint32_t tP = tmem + 128 * pass, tAcc = tP + 64;
+    const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
+    constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 64, BF, false, false),
+                       kIdescM = make_idesc(128, 64, BF, false, true);
+    auto sync = [&]() {
+      tc_fence_before_sync();
+      named_sync(1 + pass, 128);
+    };
+    auto wait = [&](uint64_t* bar, int n) { wait_bar_warp(bar, (n >> 1) & 1, abort_flag, kWaitChunkMma, n); };
+    int n = 0;
+    for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
+      const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
+      const bool with_state = lower ? has_s(chunk) : has_r(chunk);
+      const BwdInfo& f = info[s];
+      // E = dO V^T    E' = V dO^T    P' = K Q^T        rows of: K, Q, dO       result over: Q, K, V
+      unsigned char* sA = pass == 0 ? tile_o(s) : pass == 1 ? tile_v(s) : tile_k(s);
+      unsigned char* sB = pass == 0 ? tile_v(s) : pass == 1 ? tile_o(s) : tile_q(s);
+      unsigned char* sC = pass == 0 ? tile_k(s) : pass == 1 ? tile_q(s) : tile_o(s);
+      unsigned char* sOut = pass == 0 ? tile_q(s) : pass == 1 ? tile_k(s) : tile_v(s);
+      wait(&bar_full[s], n);  // (tiles are read row by row below: every reader has to see the loads' completion itself)
+      wait(&bar_ready[s], n);
+      if (wq == 0) {
+        if (elect_one() && !*abort_flag) {
+          tc_fence_after_sync();
+          const uint64_t dA = kdesc(smem_u32(sA)), dB = kdesc(smem_u32(sB));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ss(tP, dA + 2 * k, dB + 2 * k, kIdescP, k > 0);
+          mma_commit(&bar_score[pass][s]);
+          if (n > 0) {  // the store of the chunk before: its stage is free when it has been read
+            tma_store_wait_read<0>();
+            mbar_arrive(&bar_free[s ^ 1]);
+          }
+        }
+        __syncwarp();
+      }
+      const float Gr = f.G[row];
+      const float rowf = __expf(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
+      const float scale = __expf(lower ? Gr : f.G[kGtChunk - 1] - Gr);
+      const float* col = lower ? f.low[wq] : f.up[wq];
+      wait(&bar_score[pass][s], n);
+      tc_fence_after_sync();
+      // decayed, masked, packed in place: block b of 32 columns goes to 16 columns that belong to block b / 2, already read
+#pragma unroll 1
+      for (int blk = 0; blk < 4; ++blk) {
+        uint32_t pk[16];
+        if (lower ? blk > wq : blk < wq) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) pk[j] = 0u;
+        } else {
+          uint32_t r[32];
+          tmem_ld_x32(tP + lane_base + 32 * blk, r);
+          if (blk == wq) {
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 Gs = *reinterpret_cast<const float4*>(&f.G[32 * blk + j]);
+              const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * __expf(lower ? Gr - gs[e] : gs[e] - Gr) : 0.f;
+              pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
+              pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
+            }
+          } else {
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 cf = *reinterpret_cast<const float4*>(&col[32 * blk + j]);
+              pk[j / 2] = Pack2<T>::pack(__uint_as_float(r[j]) * (rowf * cf.x), __uint_as_float(r[j + 1]) * (rowf * cf.y));
+              pk[j / 2 + 1] = Pack2<T>::pack(__uint_as_float(r[j + 2]) * (rowf * cf.z), __uint_as_float(r[j + 3]) * (rowf * cf.w));
+            }
+          }
+        }
+        tmem_st_x16(tP + lane_base + 16 * blk, pk);
+      }
+      tmem_st_wait();
+      sync();
+      float across = 0.f;
+      if (with_state) {  // the state's part, into the accumulator, and scaled there
+        if (wq == 0) {
+          if (elect_one() && !*abort_flag) {
+            tc_fence_after_sync();
+            const uint64_t dA = kdesc(smem_u32(sA));
+            unsigned char* st = lower ? state_s(s) : state_r(s);
+            if (pass == 2) {
+              const uint64_t d = mdesc(smem_u32(st));
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ss(tAcc, dA + 2 * k, d + 128 * k, kIdescM, k > 0);
+            } else {
+              const uint64_t d = kdesc(smem_u32(st));
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ss(tAcc, dA + 2 * k, d + 2 * k, kIdescK, k > 0);
+            }
+            mma_commit(&bar_state[pass][s]);
+          }
+          __syncwarp();
+        }
+        wait(&bar_state[pass][s], n);
+        tc_fence_after_sync();
+#pragma unroll 1
+        for (int blk = 0; blk < 4; ++blk) {
+          uint32_t r[16];
+          tmem_ld_x16(tAcc + lane_base + 16 * blk, r);
+          uint4 u, w;
+          if (pass == 1) u = *tile_piece(tile_k(s), row, 2 * blk), w = *tile_piece(tile_k(s), row, 2 * blk + 1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
+          if (pass == 1) across += dot16<T>(r, u, w);
+          tmem_st_x16(tAcc + lane_base + 16 * blk, r);
+        }
+        tmem_st_wait();
+        sync();
+      } else if (wq == 0) {  // (the barrier has one phase per chunk, whether there is a state or not)
+        if (elect_one()) mbar_arrive(&bar_state[pass][s]);
+        __syncwarp();
+      }
+      if (wq == 0) {
+        if (elect_one() && !*abort_flag) {
+          tc_fence_after_sync();
+          const uint64_t d = mdesc(smem_u32(sC));
+          mma_ts(tAcc, tP, d, kIdescM, with_state ? 1u : 0u);
+#pragma unroll
+          for (int k = 1; k < 8; ++k) mma_ts(tAcc, tP + 8 * k, d + 128 * k, kIdescM, 1u);
+          mma_commit(&bar_rows[pass][s]);
+        }
+        __syncwarp();
+      }
+      wait(&bar_rows[pass][s], n);
+      // the other groups' MMAs that read the tile under the result
+      if (pass == 0) {
+        wait(&bar_score[2][s], n);
+        wait(&bar_rows[1][s], n);
+      } else if (pass == 1) {
+        wait(&bar_score[2][s], n);
+        wait(&bar_rows[0][s], n);
+        if (with_state) wait(&bar_state[2][s], n);
+      } else {
+        wait(&bar_score[0][s], n);
+        wait(&bar_score[1][s], n);
+        if (with_state) wait(&bar_state[1][s], n);
+      }
+      tc_fence_after_sync();
+      if (pass == 2) {
+        row_from_acc<T, false>(sOut, row, tAcc + lane_base, 1.f, 0.f);
+      } else {
+        const float dot = row_from_acc_dot<T>(sOut, row, tAcc + lane_base, 1.f);  // q.dq, k.dk: the result's row takes the place of q's, k's
+        if (pass == 0) {
+          info[s].qd[row] = dot;
+        } else {
+          info[s].kd[row] = dot - across;
+          info[s].bd[row] = across;
+        }
+        warp_arrive(&bar_dots[s], lane);
+      }
+      fence_proxy_async_smem();
+      sync();
+      if (wq == 0) {
+        if (elect_one() && !*abort_flag) {
+          const long bh = unit / a.nchunks;
+          tma_store_tile(pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv, sOut, chunk * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
+          tma_store_commit();
+        }
+        __syncwarp();
+      }
+    }
+    if (wq == 0) {
+      if (elect_one()) tma_store_wait_read<0>();
+      __syncwarp();
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) {  // no load may be in flight when the CTA leaves
+    for (int n = loads_s > 2 ? loads_s - 2 : 0; n < loads_s; ++n) mbar_wait(&bar_full[n & 1], (n >> 1) & 1, 64);
+  }
+  __syncthreads();
+  if (warp == 16) tmem_dealloc(tmem, 512);
+}
+
 }  // namespace cott

@@ -117,6 +117,12 @@ int run_tc_bwd(const GatedArgs& g, const void* states, void* ws, int B, int dtyp
   GatedChunkArgs c = chunk_args(g, bh);
   TRY((launch_walk<T, D, true>(a, m.q, m.o, bh, p + round256(c.units * tile_bytes(D)), stream)));
   c.S = static_cast<const unsigned char*>(states), c.R = a.states, c.dgate = g.dgate, c.with_last = g.dfinal != nullptr;
+  if constexpr (D == 64) {
+    auto kern = gated_bwd64_kernel<T>;
+    COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwd64Smem));
+    COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(c.units < kSms ? c.units : kSms)), kBwd64Threads, kBwd64Smem, stream, m, c));
+    return COTT_OK;
+  }
   auto kern = gated_bwd_tc_kernel<T, D>;
   COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd_tc_smem<D>()));
   COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)c.units), bwd_threads<D>(), bwd_tc_smem<D>(), stream, m, c));
