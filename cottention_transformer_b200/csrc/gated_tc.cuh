@@ -24,7 +24,8 @@ namespace cott {
 constexpr int kGtChunk = 128;
 constexpr int kStateTile = 64 * 128;      // bytes of a [64 x 64] 16-bit tile
 constexpr int kWalkThreads = 448;
-constexpr float kGateFloorTc = -200.f;    // e^-200 = 0 in fp32; sums of it keep their digits
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGateFloorTc = -200.f * kLog2e;  // e^-200 = 0 in fp32; sums of it keep their digits
 
 enum { kWaitWalkTma = 16, kWaitWalkFree = 17, kWaitWalkPrep = 18, kWaitWalkState = 19, kWaitChunkTma = 20, kWaitChunkMma = 21 };
 
@@ -40,11 +41,17 @@ struct GatedTcArgs {
   int H, N, nchunks, chunks_per_seg, nseg, gate_f32;
 };
 
+// One gate, in units of log 2 (all decays are then one ex2 away).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <typename T>
 __device__ __forceinline__ float gate_tc(const void* gate, const unsigned char* keep, const cott_strides& sg, int gate_f32, int N, long b, int h, int pos) {
   if (pos >= N || (keep && !keep[b * N + pos])) return 0.f;
   const long long o = b * sg.b + h * sg.h + static_cast<long long>(pos) * sg.n;
-  const float g = gate_f32 ? static_cast<const float*>(gate)[o] : to_acc(static_cast<const T*>(gate)[o]);
+  const float g = kLog2e * (gate_f32 ? static_cast<const float*>(gate)[o] : to_acc(static_cast<const T*>(gate)[o]));
   return g < kGateFloorTc ? kGateFloorTc : g;
 }
 // Four consecutive gates a lane -> their inclusive sums over the chunk, from its start or (SUFFIX) the sums of what comes after each of
@@ -221,7 +228,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
         const float x = __shfl_sync(0xffffffffu, g[e], 8 * wq + (lane >> 2));
         if ((lane & 3) == e) G = x;
       }
-      const float w = __expf(G);
+      const float w = ex2(G);
       const bool take = kp;
       if (c + 2 < updates) fetch(c + 2);
       if (!wait_bar_warp(&bar_full[s], (c / NS) & 1, abort_flag, kWaitWalkTma, c)) break;
@@ -299,7 +306,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       float total = (g[0] + g[1]) + (g[2] + g[3]);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-      const float A = __expf(total);
+      const float A = ex2(total);
       log_sum += total;
       if (c + 1 < updates) fetch(c + 1);
       if (!(ok = wait_bar_warp(&bar_u_full[c & 1], (c >> 1) & 1, abort_flag, kWaitWalkState, c))) break;
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(256) gated_seg_kernel(const GatedTcArgs a) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       x[u] = s + u < a.nseg ? p[static_cast<long>(s + u) * (D * 64)] : 0.f;
-      d[u] = s + u < a.nseg ? __expf(lg[s + u]) : 1.f;
+      d[u] = s + u < a.nseg ? ex2(lg[s + u]) : 1.f;
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -396,7 +403,14 @@ __device__ __forceinline__ void chunk_gates(const GatedChunkArgs& a, float* sG, 
 }
 template <bool LOWER>
 __device__ __forceinline__ void col_factor(float (*sCol)[kGtChunk], const float* sG, int w, int s) {
-  if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = __expf(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
+  if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = ex2(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {  // two products in one instruction
+  float2 c;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
 }
 // 32 columns (block `blk`) of the scores of a row of block wq, decayed, masked and packed
 template <typename T, bool LOWER>
@@ -419,7 +433,7 @@ __device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_l
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool in = LOWER ? j + e <= lane : j + e >= lane;
-        x[e] = in ? __uint_as_float(r[j + e]) * __expf(LOWER ? Gr - gs[e] : gs[e] - Gr) : 0.f;
+        x[e] = in ? __uint_as_float(r[j + e]) * ex2(LOWER ? Gr - gs[e] : gs[e] - Gr) : 0.f;
       }
       pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
       pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
@@ -569,7 +583,7 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   }
   wait_bar_warp(&bar_mma[0], 0, abort_flag, kWaitChunkMma, chunk);
   tc_fence_after_sync();
-  const float Gr = sG[row], rowf = __expf(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f);
+  const float Gr = sG[row], rowf = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f);
   uint32_t pk[2][16];
 #pragma unroll
   for (int i = 0; i < 2; ++i) decay_block<T, true>(pk[i], tP + lane_base, 2 * hf + i, wq, lane, Gr, rowf, sG, sCol[wq]);
@@ -593,7 +607,7 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   if (with_state) {
     wait_bar_warp(&bar_mma[1], 0, abort_flag, kWaitChunkMma, chunk);
     tc_fence_after_sync();
-    acc_scaled(acc, tAcc + lane_base + 32 * hf, __expf(Gr));
+    acc_scaled(acc, tAcc + lane_base + 32 * hf, ex2(Gr));
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) acc[j] = 0.f;
@@ -794,8 +808,8 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
     scores(tY, dV, dO, &bar_score[1]);
   });
   const float Gr = sG[row], total = sG[kGtChunk - 1];
-  const float head = __expf(Gr), tail = __expf(total - Gr);
-  const float row_low = __expf(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = __expf(sG[32 * wq + 31] - Gr);
+  const float head = ex2(Gr), tail = ex2(total - Gr);
+  const float row_low = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = ex2(sG[32 * wq + 31] - Gr);
   const int panel = cg / 2 * kTileBytes, j0 = 4 * (cg & 1);  // where this thread's 32 columns are in a row of D
 
   uint32_t pk[NB][16];
@@ -930,7 +944,7 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
     float sr = 0.f;
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) sr += sCross[i];
-    const float A = __expf(total);
+    const float A = ex2(total);
     x += A == 0.f ? 0.f : A * sr;
     for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
     const int pos = c0 + row;
@@ -945,24 +959,26 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
 }
 
 // ---- backward at head dim 64: a persistent kernel ------------------------------------------------------------------------
-// The same three passes, a group of four warps for each, side by side.  A thread owns a row, so that scores are decayed and packed
-// in place without a word to the other warps, and everything a group does per chunk is a handful of rolled loops that all three run
-// (the one-chunk kernel spent a quarter of its time waiting for instructions and another at its barriers):
+// The same three passes, a group of eight warps for each, side by side.  A thread owns half a row, and each half is packed in place
+// and has its half of the accumulator beside it, so that a warp reads what it alone has written over; everything a group does per
+// chunk is a handful of rolled loops that all three run (the one-chunk kernel spent a quarter of its time waiting for instructions
+// and another at its barriers):
 //     scores (MMA) -> decay, pack -> state's part (MMA) -> scale -> rows (MMA) -> result over a tile -> TMA
-//   warps 0-3: dq over Q     4-7: dk over K     8-11: dv over V     (rows and TMEM lanes 32 (w % 4) ..)
-//   warps 12-15: gates of the next chunk, masked rows, <S, R>, dg   warp 16: TMA loads
-// Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group: scores, then the packed scores and the accumulator.
+//   warps 0-7: dq over Q     8-15: dk over K     16-23: dv over V     (rows and TMEM lanes 32 (w % 4) .., half (w / 4) % 2)
+//   warps 24-27: gates of the next chunk, masked rows, <S, R>, dg     warp 28: TMA loads
+// Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and
+// 32 of the accumulator.
 // A result is staged over a tile when the MMAs that read it have completed, whichever group issued them; the barriers for that are
 // kept per stage, so that nobody can be a whole phase ahead of one that is still waiting.
 // Every wait is bounded.  After one that gave up, nothing more is issued, every further wait returns at once and all warps still go
 // through all named barriers.
-constexpr int kBwd64Threads = 544;
+constexpr int kBwd64Threads = 928;
 constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
 constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
 
 struct __align__(16) BwdInfo {  // of a stage's chunk
   float G[kGtChunk], low[4][kGtChunk], up[4][kGtChunk];
-  float gate[kGtChunk], qd[kGtChunk], kd[kGtChunk], bd[kGtChunk];
+  float gate[kGtChunk], qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];  // (the dot products by halves)
 };
 
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -997,7 +1013,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       mbar_init(&bar_full[s], 1);
       mbar_init(&bar_free[s], 7);   // three stores, four warps that took <S, R>
       mbar_init(&bar_ready[s], 4);
-      mbar_init(&bar_dots[s], 8);
+      mbar_init(&bar_dots[s], 16);
       for (int p = 0; p < 3; ++p) {
         mbar_init(&bar_score[p][s], 1);
         mbar_init(&bar_state[p][s], 1);
@@ -1012,7 +1028,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     tma_prefetch_desc(&m.v);
     tma_prefetch_desc(&m.o);
   }
-  if (warp == 16) {
+  if (warp == 28) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
@@ -1023,7 +1039,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   pdl_wait_prior();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 16) {
+  if (warp == 28) {
     // ---------------------------------------------------------------- loads
     if (elect_one()) {
       int n = 0;
@@ -1042,9 +1058,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         loads_s = n + 1;
       }
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 24) {
     // ---------------------------------------------------------------- gates, masked rows, <S, R>, dg
-    const int t = tid - 384;  // position
+    const int t = tid - 768;  // position
     float g[4], gt = 0.f, cross_before = 0.f;
     bool kp = true, kp_before = true;
     auto fetch = [&](long unit) {
@@ -1061,7 +1077,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       wait_bar_warp(&bar_dots[n & 1], (n >> 1) & 1, abort_flag, kWaitAcc, n);
       const long bh = u / a.nchunks, b = bh / a.H;
       const int chunk = static_cast<int>(u % a.nchunks), h = static_cast<int>(bh % a.H), pos = chunk * kGtChunk + t;
-      float run = f.qd[t] - f.kd[t], up = f.bd[t];
+      float run = (f.qd[0][t] + f.qd[1][t]) - (f.kd[0][t] + f.kd[1][t]), up = f.bd[0][t] + f.bd[1][t];
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {  // run: from the row to the warp's end; up: to the row
         const float d = __shfl_down_sync(0xffffffffu, run, off), x = __shfl_up_sync(0xffffffffu, up, off);
@@ -1073,7 +1089,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       if (lane == 31) sPart[4 + wq] = up;
       const float before = __shfl_up_sync(0xffffffffu, up, 1);
       named_sync(4, 128);
-      const float A = __expf(f.G[kGtChunk - 1]);
+      const float A = ex2(f.G[kGtChunk - 1]);
       float x = run + (lane ? before : 0.f) + (A == 0.f ? 0.f : A * ((sPart[8] + sPart[9]) + (sPart[10] + sPart[11])));
       for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
       if (pos < a.N && !*abort_flag) {
@@ -1137,15 +1153,16 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
   } else {
     // ---------------------------------------------------------------- the passes
-    const int pass = warp >> 2;  // 0 dq, 1 dk, 2 dv
-    const bool lower = pass == 0;
-    const uint32_t tP = tmem + 128 * pass, tAcc = tP + 64;
+    const int pass = warp >> 3, half = (warp >> 2) & 1;  // 0 dq, 1 dk, 2 dv
+    const bool lower = pass == 0, issuer = (warp & 7) == 0;
+    const uint32_t tP = tmem + 128 * pass, tMine = tP + 64 * half + lane_base;
+    const float sign = lower ? 1.f : -1.f;
     const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
-    constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 64, BF, false, false),
-                       kIdescM = make_idesc(128, 64, BF, false, true);
+    constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 32, BF, false, false),
+                       kIdescM = make_idesc(128, 32, BF, false, true);
     auto sync = [&]() {
       tc_fence_before_sync();
-      named_sync(1 + pass, 128);
+      named_sync(1 + pass, 256);
     };
     auto wait = [&](uint64_t* bar, int n) { wait_bar_warp(bar, (n >> 1) & 1, abort_flag, kWaitChunkMma, n); };
     int n = 0;
@@ -1160,7 +1177,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       unsigned char* sOut = pass == 0 ? tile_q(s) : pass == 1 ? tile_k(s) : tile_v(s);
       wait(&bar_full[s], n);  // (tiles are read row by row below: every reader has to see the loads' completion itself)
       wait(&bar_ready[s], n);
-      if (wq == 0) {
+      if (issuer) {
         if (elect_one() && !*abort_flag) {
           tc_fence_after_sync();
           const uint64_t dA = kdesc(smem_u32(sA)), dB = kdesc(smem_u32(sB));
@@ -1175,63 +1192,68 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         __syncwarp();
       }
       const float Gr = f.G[row];
-      const float rowf = __expf(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
-      const float scale = __expf(lower ? Gr : f.G[kGtChunk - 1] - Gr);
+      const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
+      const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
       const float* col = lower ? f.low[wq] : f.up[wq];
       wait(&bar_score[pass][s], n);
       tc_fence_after_sync();
-      // decayed, masked, packed in place: block b of 32 columns goes to 16 columns that belong to block b / 2, already read
+      // decayed, masked, packed in place: the half's first 32 columns into its first 16, then the others into the next 16
 #pragma unroll 1
-      for (int blk = 0; blk < 4; ++blk) {
+      for (int i = 0; i < 2; ++i) {
+        const int blk = 2 * half + i;
         uint32_t pk[16];
         if (lower ? blk > wq : blk < wq) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) pk[j] = 0u;
         } else {
           uint32_t r[32];
-          tmem_ld_x32(tP + lane_base + 32 * blk, r);
+          tmem_ld_x32(tMine + 32 * i, r);
+          tmem_ld_wait();
           if (blk == wq) {
-            tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 Gs = *reinterpret_cast<const float4*>(&f.G[32 * blk + j]);
               const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
               float x[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * __expf(lower ? Gr - gs[e] : gs[e] - Gr) : 0.f;
+              for (int e = 0; e < 4; ++e) x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * ex2(sign * (Gr - gs[e])) : 0.f;
               pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
               pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
             }
           } else {
-            tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 cf = *reinterpret_cast<const float4*>(&col[32 * blk + j]);
-              pk[j / 2] = Pack2<T>::pack(__uint_as_float(r[j]) * (rowf * cf.x), __uint_as_float(r[j + 1]) * (rowf * cf.y));
-              pk[j / 2 + 1] = Pack2<T>::pack(__uint_as_float(r[j + 2]) * (rowf * cf.z), __uint_as_float(r[j + 3]) * (rowf * cf.w));
+              const float2 x = mul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2(make_float2(cf.x, cf.y), make_float2(rowf, rowf)));
+              const float2 y = mul2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), mul2(make_float2(cf.z, cf.w), make_float2(rowf, rowf)));
+              pk[j / 2] = Pack2<T>::pack(x.x, x.y);
+              pk[j / 2 + 1] = Pack2<T>::pack(y.x, y.y);
             }
           }
         }
-        tmem_st_x16(tP + lane_base + 16 * blk, pk);
+        tmem_st_x16(tMine + 16 * i, pk);
       }
       tmem_st_wait();
       sync();
       float across = 0.f;
       if (with_state) {  // the state's part, into the accumulator, and scaled there
-        if (wq == 0) {
+        if (issuer) {
           if (elect_one() && !*abort_flag) {
             tc_fence_after_sync();
             const uint64_t dA = kdesc(smem_u32(sA));
             unsigned char* st = lower ? state_s(s) : state_r(s);
-            if (pass == 2) {
+            if (pass == 2) {  // columns 32 hh .. of R: 64 bytes into its rows
               const uint64_t d = mdesc(smem_u32(st));
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss(tAcc, dA + 2 * k, d + 128 * k, kIdescM, k > 0);
-            } else {
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 4 * hh + 128 * k, kIdescM, k > 0);
+            } else {  // rows 32 hh .. of S, R
               const uint64_t d = kdesc(smem_u32(st));
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss(tAcc, dA + 2 * k, d + 2 * k, kIdescK, k > 0);
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 256 * hh + 2 * k, kIdescK, k > 0);
             }
             mma_commit(&bar_state[pass][s]);
           }
@@ -1240,30 +1262,32 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         wait(&bar_state[pass][s], n);
         tc_fence_after_sync();
 #pragma unroll 1
-        for (int blk = 0; blk < 4; ++blk) {
+        for (int i = 0; i < 2; ++i) {
           uint32_t r[16];
-          tmem_ld_x16(tAcc + lane_base + 16 * blk, r);
+          tmem_ld_x16(tMine + 32 + 16 * i, r);
           uint4 u, w;
-          if (pass == 1) u = *tile_piece(tile_k(s), row, 2 * blk), w = *tile_piece(tile_k(s), row, 2 * blk + 1);
+          if (pass == 1) u = *tile_piece(tile_k(s), row, 4 * half + 2 * i), w = *tile_piece(tile_k(s), row, 4 * half + 2 * i + 1);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
           if (pass == 1) across += dot16<T>(r, u, w);
-          tmem_st_x16(tAcc + lane_base + 16 * blk, r);
+          tmem_st_x16(tMine + 32 + 16 * i, r);
         }
         tmem_st_wait();
         sync();
-      } else if (wq == 0) {  // (the barrier has one phase per chunk, whether there is a state or not)
+      } else if (issuer) {  // (the barrier has one phase per chunk, whether there is a state or not)
         if (elect_one()) mbar_arrive(&bar_state[pass][s]);
         __syncwarp();
       }
-      if (wq == 0) {
+      if (issuer) {
         if (elect_one() && !*abort_flag) {
           tc_fence_after_sync();
           const uint64_t d = mdesc(smem_u32(sC));
-          mma_ts(tAcc, tP, d, kIdescM, with_state ? 1u : 0u);
 #pragma unroll
-          for (int k = 1; k < 8; ++k) mma_ts(tAcc, tP + 8 * k, d + 128 * k, kIdescM, 1u);
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              mma_ts(tP + 64 * hh + 32, tP + 8 * (k & 3) + 64 * (k >> 2), d + 4 * hh + 128 * k, kIdescM, k > 0 || with_state ? 1u : 0u);
           mma_commit(&bar_rows[pass][s]);
         }
         __syncwarp();
@@ -1283,21 +1307,35 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         if (with_state) wait(&bar_state[1][s], n);
       }
       tc_fence_after_sync();
-      if (pass == 2) {
-        row_from_acc<T, false>(sOut, row, tAcc + lane_base, 1.f, 0.f);
-      } else {
-        const float dot = row_from_acc_dot<T>(sOut, row, tAcc + lane_base, 1.f);  // q.dq, k.dk: the result's row takes the place of q's, k's
+      float dot = 0.f;  // q.dq, k.dk over the half's columns; the result's row takes the place of q's, k's
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        uint32_t r[16];
+        tmem_ld_x16(tMine + 32 + 16 * i, r);
+        uint4 *p0 = tile_piece(sOut, row, 4 * half + 2 * i), *p1 = tile_piece(sOut, row, 4 * half + 2 * i + 1);
+        uint4 u, w;
+        if (pass < 2) u = *p0, w = *p1;
+        tmem_ld_wait();
+        if (pass < 2) dot += dot16<T>(r, u, w);
+        u.x = Pack2<T>::pack(__uint_as_float(r[0]), __uint_as_float(r[1])), u.y = Pack2<T>::pack(__uint_as_float(r[2]), __uint_as_float(r[3]));
+        u.z = Pack2<T>::pack(__uint_as_float(r[4]), __uint_as_float(r[5])), u.w = Pack2<T>::pack(__uint_as_float(r[6]), __uint_as_float(r[7]));
+        w.x = Pack2<T>::pack(__uint_as_float(r[8]), __uint_as_float(r[9])), w.y = Pack2<T>::pack(__uint_as_float(r[10]), __uint_as_float(r[11]));
+        w.z = Pack2<T>::pack(__uint_as_float(r[12]), __uint_as_float(r[13])), w.w = Pack2<T>::pack(__uint_as_float(r[14]), __uint_as_float(r[15]));
+        *p0 = u;
+        *p1 = w;
+      }
+      if (pass < 2) {
         if (pass == 0) {
-          info[s].qd[row] = dot;
+          info[s].qd[half][row] = dot;
         } else {
-          info[s].kd[row] = dot - across;
-          info[s].bd[row] = across;
+          info[s].kd[half][row] = dot - across;
+          info[s].bd[half][row] = across;
         }
         warp_arrive(&bar_dots[s], lane);
       }
       fence_proxy_async_smem();
       sync();
-      if (wq == 0) {
+      if (issuer) {
         if (elect_one() && !*abort_flag) {
           const long bh = unit / a.nchunks;
           tma_store_tile(pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv, sOut, chunk * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
@@ -1306,7 +1344,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         __syncwarp();
       }
     }
-    if (wq == 0) {
+    if (issuer) {
       if (elect_one()) tma_store_wait_read<0>();
       __syncwarp();
     }
@@ -1319,7 +1357,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     for (int n = loads_s > 2 ? loads_s - 2 : 0; n < loads_s; ++n) mbar_wait(&bar_full[n & 1], (n >> 1) & 1, 64);
   }
   __syncthreads();
-  if (warp == 16) tmem_dealloc(tmem, 512);
+  if (warp == 28) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace cott
