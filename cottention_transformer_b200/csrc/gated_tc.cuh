@@ -76,8 +76,9 @@ __device__ __forceinline__ float gate_tc(const void* gate, const unsigned char* 
 // Four consecutive gates a lane -> their inclusive sums over the chunk, from its start or (SUFFIX) the sums of what comes after each of
 // them; the whole warp takes part.  Additions only: a difference of two sums that both contain a dropped state would leave the
 // short sums beside it few digits.
+// Returns the sum of all.
 template <bool SUFFIX>
-__device__ __forceinline__ void gate_sums(float (&g)[4], int lane) {
+__device__ __forceinline__ float gate_sums(float (&g)[4], int lane) {
   if constexpr (SUFFIX) {
     const float g3 = g[3], g32 = g[2] + g3, g321 = g[1] + g32;
     float run = g[0] + g321;
@@ -89,6 +90,7 @@ __device__ __forceinline__ void gate_sums(float (&g)[4], int lane) {
     float after = __shfl_down_sync(0xffffffffu, run, 1);
     if (lane == 31) after = 0.f;
     g[3] = after, g[2] = after + g3, g[1] = after + g32, g[0] = after + g321;
+    return __shfl_sync(0xffffffffu, run, 0);
   } else {
     g[1] += g[0], g[2] += g[1], g[3] += g[2];
     float run = g[3];
@@ -101,7 +103,24 @@ __device__ __forceinline__ void gate_sums(float (&g)[4], int lane) {
     if (lane == 0) before = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) g[e] += before;
+    return __shfl_sync(0xffffffffu, run, 31);
   }
+}
+
+// Two barriers at once for a whole warp: one round trip instead of two.
+__device__ __forceinline__ bool wait_bar2_warp(uint64_t* bar_a, uint32_t parity_a, uint64_t* bar_b, uint32_t parity_b, volatile int* abort_flag, int code,
+                                               int chunk) {
+  bool ok = false;
+  for (uint32_t i = 0; i < ptx::kMaxPolls && !ok; ++i) {
+    const bool a = ptx::mbar_try_wait(bar_a, parity_a), b = ptx::mbar_try_wait(bar_b, parity_b);
+    ok = __all_sync(0xffffffffu, a && b);
+    if (!ok && *abort_flag) return false;
+  }
+  if (!ok) {
+    *abort_flag = 1;
+    atomicCAS(&g_cott_status, 0, (code << 16) | (chunk & 0xffff));
+  }
+  return ok;
 }
 
 __device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
@@ -114,19 +133,40 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 }
 
 // One 16-byte piece scaled by w, as a sum of SPLIT 16-bit numbers: each takes what the ones before it have left.
+// bf16 in two numbers stays in packed 16-bit arithmetic, four instructions a pair instead of ten: with w = wh + wl, t = x wl,
+// head = x wh + t, and x wh - head is a number of few bits, which t completes.  (float16 has too little range to hold the factor.)
+template <typename T> struct Factor {
+  float w;
+  typename Vec2<T>::type hi, lo;
+  __device__ __forceinline__ explicit Factor(float f) : w(f) {
+    const float h = Vec2<T>::head(f);
+    hi = Vec2<T>::bcast(h), lo = Vec2<T>::bcast(f - h);
+  }
+};
 template <typename T, int SPLIT>
-__device__ __forceinline__ void scale_split(const uint4& u, uint4 (&out)[SPLIT], float w) {
-  const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void scale_split(const uint4& u, uint4 (&out)[SPLIT], const Factor<T>& f) {
+  if constexpr (SPLIT == 2 && Pack2<T>::kBf16) {
+    using V = typename Vec2<T>::type;
+    const V* x = reinterpret_cast<const V*>(&u);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float2 f = Pack2<T>::unpack(x[e]);
-    f.x *= w, f.y *= w;
+    for (int e = 0; e < 4; ++e) {
+      const V t = __hmul2(x[e], f.lo), h = __hfma2(x[e], f.hi, t);
+      reinterpret_cast<V*>(&out[0])[e] = h;
+      reinterpret_cast<V*>(&out[1])[e] = __hadd2(__hfma2(x[e], f.hi, __hneg2(h)), t);
+    }
+  } else {
+    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < SPLIT; ++i) {
-      const uint32_t p = Pack2<T>::pack(f.x, f.y);
-      reinterpret_cast<uint32_t*>(&out[i])[e] = p;
-      const float2 h = Pack2<T>::unpack(p);
-      f.x -= h.x, f.y -= h.y;
+    for (int e = 0; e < 4; ++e) {
+      float2 y = Pack2<T>::unpack(x[e]);
+      y.x *= f.w, y.y *= f.w;
+#pragma unroll
+      for (int i = 0; i < SPLIT; ++i) {
+        const uint32_t p = Pack2<T>::pack(y.x, y.y);
+        reinterpret_cast<uint32_t*>(&out[i])[e] = p;
+        const float2 h = Pack2<T>::unpack(p);
+        y.x -= h.x, y.y -= h.y;
+      }
     }
   }
 }
@@ -152,7 +192,11 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* sOut = smem + NS * STAGE;  // 2 x NT state tiles on their way out
-  __shared__ uint64_t bar_full[NS], bar_free[NS], bar_prep[NS], bar_u_full[2], bar_u_free[2];
+  // (sums of the gates: the operand warps are at most NS + 2 chunks ahead of the state warps)
+  constexpr int NSUM = 8;
+  static_assert(NS + 2 < NSUM, "a sum is read before its place is taken again");
+  __shared__ uint64_t bar_full[NS], bar_free[NS], bar_prep[NS], bar_u_full[2], bar_u_free[2], bar_sum[NSUM];
+  __shared__ float sSum[NSUM];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
   volatile int* abort_flag = &abort_flag_s;
@@ -176,6 +220,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       mbar_init(&bar_u_full[i], 1);
       mbar_init(&bar_u_free[i], 4);
     }
+    for (int i = 0; i < NSUM; ++i) mbar_init(&bar_sum[i], 1);
     mbar_fence_init();
     abort_flag_s = 0;
     tma_prefetch_desc(&mapY);
@@ -227,11 +272,18 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     const int wq = warp & 3, row = 32 * wq + lane, mine = warp >= 10 ? 1 : 0;
     RawGate raw[4];
     unsigned char kp = 1;
+    const long long g0 = b * a.sg.b + h * a.sg.h + 4 * lane * a.sg.n;
+    const unsigned char* keep_b = a.keep ? a.keep + b * a.N : nullptr;
     auto fetch = [&](int c) {
       const int p0 = chunk_at(c) * kGtChunk;
+      const long long o = g0 + p0 * a.sg.n;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) raw[e] = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, p0 + 4 * lane + e);
-      if (a.keep) kp = p0 + row < a.N ? a.keep[b * a.N + p0 + row] : 0;
+      for (int e = 0; e < 4; ++e) {
+        const bool in = p0 + 4 * lane + e < a.N;
+        raw[e].bits = !in ? 0u : a.gate_f32 ? static_cast<const uint32_t*>(a.gate)[o + e * a.sg.n] : static_cast<const unsigned short*>(a.gate)[o + e * a.sg.n];
+        raw[e].take = !in ? 0 : keep_b ? keep_b[p0 + 4 * lane + e] : 1;
+      }
+      if (keep_b) kp = p0 + row < a.N ? keep_b[p0 + row] : 0;
     };
     if (updates > mine) fetch(mine);
     for (int c = 0; c < updates; ++c) {
@@ -243,14 +295,18 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       float g[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) g[e] = gate_of<T>(raw[e], a.gate_f32);
-      gate_sums<!REV>(g, lane);  // G_last - G_s, or G_t
+      const float total = gate_sums<!REV>(g, lane);  // G_last - G_s, or G_t
+      if (wq == 0 && lane == 0) {
+        sSum[c % NSUM] = total;
+        mbar_arrive(&bar_sum[c % NSUM]);
+      }
       float G = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = __shfl_sync(0xffffffffu, g[e], 8 * wq + (lane >> 2));
         if ((lane & 3) == e) G = x;
       }
-      const float w = ex2(G);
+      const Factor<T> w(ex2(G));
       const bool take = kp != 0;
       if (c + 2 < updates) fetch(c + 2);
       if (!wait_bar_warp(&bar_full[s], (c / NS) & 1, abort_flag, kWaitWalkTma, c)) break;
@@ -292,13 +348,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
 #pragma unroll
       for (int j = 0; j < 64; ++j) S[j] = a.edge[edge + static_cast<long>(j) * D];
     }
-    RawGate raw[4];
     float log_sum = 0.f;
-    auto fetch = [&](int c) {
-      const int p0 = chunk_at(c) * kGtChunk;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) raw[e] = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, p0 + 4 * lane + e);
-    };
     auto emit = [&](int slot, int n) {  // n: how many were emitted before
       unsigned char* panel = sOut + (n & 1) * NT * kStateTile;
       if (lane == 0) tma_store_wait_read<1>();  // the copy of two emissions ago has left the buffer
@@ -321,18 +371,13 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
         tma_store_commit();
       }
     };
-    if (updates > 0) fetch(0);
     bool ok = true;
     for (int c = 0; c < nchunks; ++c) {
       if (EMIT) emit(chunk_at(c), c);
       if (c >= updates) break;
-      float total = (gate_of<T>(raw[0], a.gate_f32) + gate_of<T>(raw[1], a.gate_f32)) + (gate_of<T>(raw[2], a.gate_f32) + gate_of<T>(raw[3], a.gate_f32));
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-      const float A = ex2(total);
+      if (!(ok = wait_bar2_warp(&bar_u_full[c & 1], (c >> 1) & 1, &bar_sum[c % NSUM], (c / NSUM) & 1, abort_flag, kWaitWalkState, c))) break;
+      const float total = sSum[c % NSUM], A = ex2(total);
       log_sum += total;
-      if (c + 1 < updates) fetch(c + 1);
-      if (!(ok = wait_bar_warp(&bar_u_full[c & 1], (c >> 1) & 1, abort_flag, kWaitWalkState, c))) break;
       tc_fence_after_sync();
       if (A == 0.f) {  // a state that is dropped is dropped whatever it holds
 #pragma unroll
