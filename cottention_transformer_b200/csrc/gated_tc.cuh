@@ -1034,13 +1034,15 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
 //     scores (MMA) -> decay, pack -> state's part (MMA) -> scale -> rows (MMA) -> result over a tile -> TMA
 //   warps 0-7: dq over Q     8-15: dk over K     16-23: dv over V     (rows and TMEM lanes 32 (w % 4) .., half (w / 4) % 2)
 //   warps 24-27: gates of the next chunk, masked rows, <S, R>, dg     warp 28: TMA loads
+//   warps 29-31, one thread each: the MMAs and the stores of a pass, so that the scores of the next chunk are under way while the
+//   last rows of this one are written, and no working warp spends its time on issuing
 // Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and
 // 32 of the accumulator.
 // A result is staged over a tile when the MMAs that read it have completed, whichever group issued them; the barriers for that are
 // kept per stage, so that nobody can be a whole phase ahead of one that is still waiting.
-// Every wait is bounded.  After one that gave up, nothing more is issued, every further wait returns at once and all warps still go
-// through all named barriers.
-constexpr int kBwd64Threads = 928;
+// Every wait is bounded.  After one that gave up every further wait returns at once; the warps that share a named barrier go through
+// all of them all the same.
+constexpr int kBwd64Threads = 1024;
 constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
 constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
 
@@ -1059,6 +1061,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ BwdInfo info[2];
   __shared__ uint64_t bar_full[2], bar_free[2], bar_ready[2], bar_dots[2], bar_score[3][2], bar_state[3][2], bar_rows[3][2];
+  __shared__ uint64_t bar_packed[3], bar_scaled[3], bar_read[3], bar_staged[3];  // a group to its issuing thread, once per chunk each
   __shared__ uint32_t tmem_slot;
   __shared__ float sPart[12];
   __shared__ int abort_flag_s, loads_s;
@@ -1088,6 +1091,12 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         mbar_init(&bar_rows[p][s], 1);
       }
     }
+    for (int p = 0; p < 3; ++p) {
+      mbar_init(&bar_packed[p], 8);
+      mbar_init(&bar_scaled[p], 8);
+      mbar_init(&bar_read[p], 8);
+      mbar_init(&bar_staged[p], 8);
+    }
     mbar_fence_init();
     abort_flag_s = 0;
     loads_s = 0;
@@ -1107,7 +1116,76 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   pdl_wait_prior();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 28) {
+  // E = dO V^T    E' = V dO^T    P' = K Q^T        rows of: K, Q, dO       result over: Q, K, V
+  auto tile_of = [&](int s, int which) { return smem + s * kBwd64Stage + which * kTileBytes; };  // O 0, V 1, K 2, Q 3
+  auto tile_a = [&](int s, int pass) { return tile_of(s, pass); };
+  auto tile_b = [&](int s, int pass) { return tile_of(s, pass == 0 ? 1 : pass == 1 ? 0 : 3); };
+  auto tile_c = [&](int s, int pass) { return tile_of(s, pass == 0 ? 2 : pass == 1 ? 3 : 0); };
+  auto tile_out = [&](int s, int pass) { return tile_of(s, 3 - pass); };
+
+  if (warp >= 29) {
+    // ---------------------------------------------------------------- MMAs and stores of a pass
+    const int pass = warp - 29;
+    if (elect_one()) {
+      constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 32, BF, false, false),
+                         kIdescM = make_idesc(128, 32, BF, false, true);
+      const uint32_t tP = tmem + 128 * pass;
+      const CUtensorMap* out = pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv;
+      auto store = [&](long unit, int n) {  // the result of the n-th chunk; its stage is free when it has been read
+        if (!wait_bar1(&bar_staged[pass], n & 1, abort_flag, kWaitAcc, n)) return false;
+        const long bh = unit / a.nchunks;
+        tma_store_tile(out, tile_out(n & 1, pass), static_cast<int>(unit % a.nchunks) * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
+        tma_store_commit();
+        tma_store_wait_read<0>();
+        mbar_arrive(&bar_free[n & 1]);
+        return true;
+      };
+      int n = 0;
+      bool ok = true;
+      long unit = blockIdx.x;
+      for (; unit < a.units; unit += gridDim.x, ++n) {
+        const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
+        const bool with_state = pass == 0 ? has_s(chunk) : has_r(chunk);
+        const uint64_t dA = kdesc(smem_u32(tile_a(s, pass))), dB = kdesc(smem_u32(tile_b(s, pass)));
+        if (!(ok = wait_bar2(&bar_ready[s], (n >> 1) & 1, n > 0 ? &bar_read[pass] : &bar_ready[s], n > 0 ? (n - 1) & 1 : 0, abort_flag, kWaitChunkTma, n))) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_ss(tP, dA + 2 * k, dB + 2 * k, kIdescP, k > 0);
+        mma_commit(&bar_score[pass][s]);
+        if (n > 0 && !(ok = store(unit - gridDim.x, n - 1))) break;
+        if (!(ok = wait_bar1(&bar_packed[pass], n & 1, abort_flag, kWaitScoreReady, n))) break;
+        if (with_state) {  // the state's part, into the accumulator
+          tc_fence_after_sync();
+          if (pass == 2) {  // columns 32 hh .. of R: 64 bytes into its rows
+            const uint64_t d = mdesc(smem_u32(state_r(s)));
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 4 * hh + 128 * k, kIdescM, k > 0);
+          } else {  // rows 32 hh .. of S, R
+            const uint64_t d = kdesc(smem_u32(pass == 0 ? state_s(s) : state_r(s)));
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 256 * hh + 2 * k, kIdescK, k > 0);
+          }
+          mma_commit(&bar_state[pass][s]);
+        } else {
+          mbar_arrive(&bar_state[pass][s]);  // (one phase per chunk, whether there is a state or not; bar_scaled likewise)
+        }
+        if (!(ok = wait_bar1(&bar_scaled[pass], n & 1, abort_flag, kWaitScoreReady, n))) break;
+        tc_fence_after_sync();
+        const uint64_t d = mdesc(smem_u32(tile_c(s, pass)));
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_ts(tP + 64 * hh + 32, tP + 8 * (k & 3) + 64 * (k >> 2), d + 4 * hh + 128 * k, kIdescM, k > 0 || with_state ? 1u : 0u);
+        mma_commit(&bar_rows[pass][s]);
+      }
+      if (ok && n > 0) store(unit - gridDim.x, n - 1);
+    }
+  } else if (warp == 28) {
     // ---------------------------------------------------------------- loads
     if (elect_one()) {
       int n = 0;
@@ -1225,49 +1303,34 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   } else {
     // ---------------------------------------------------------------- the passes
     const int pass = warp >> 3, half = (warp >> 2) & 1;  // 0 dq, 1 dk, 2 dv
-    const bool lower = pass == 0, issuer = (warp & 7) == 0;
-    const uint32_t tP = tmem + 128 * pass, tMine = tP + 64 * half + lane_base;
+    const bool lower = pass == 0;
+    const uint32_t tMine = tmem + 128 * pass + 64 * half + lane_base;
     const float sign = lower ? 1.f : -1.f;
     const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
-    constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 32, BF, false, false),
-                       kIdescM = make_idesc(128, 32, BF, false, true);
-    auto sync = [&]() {
-      tc_fence_before_sync();
-      named_sync(1 + pass, 256);
+    // up to four barriers at once: one round trip
+    auto wait4 = [&](uint64_t* b0, uint64_t* b1, uint64_t* b2, uint64_t* b3, int n) {
+      const uint32_t parity = (n >> 1) & 1;
+      for (uint32_t i = 0; i < kMaxPolls; ++i) {
+        const bool d0 = mbar_try_wait(b0, parity), d1 = mbar_try_wait(b1, parity), d2 = mbar_try_wait(b2, parity), d3 = mbar_try_wait(b3, parity);
+        if (__all_sync(0xffffffffu, d0 && d1 && d2 && d3)) return true;
+        if (*abort_flag) return false;
+      }
+      *abort_flag = 1;
+      atomicCAS(&g_cott_status, 0, (kWaitChunkMma << 16) | (n & 0xffff));
+      return false;
     };
-    auto wait = [&](uint64_t* bar, int n) { wait_bar_warp(bar, (n >> 1) & 1, abort_flag, kWaitChunkMma, n); };
     int n = 0;
     for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
       const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
       const bool with_state = lower ? has_s(chunk) : has_r(chunk);
-      const BwdInfo& f = info[s];
-      // E = dO V^T    E' = V dO^T    P' = K Q^T        rows of: K, Q, dO       result over: Q, K, V
-      unsigned char* sA = pass == 0 ? tile_o(s) : pass == 1 ? tile_v(s) : tile_k(s);
-      unsigned char* sB = pass == 0 ? tile_v(s) : pass == 1 ? tile_o(s) : tile_q(s);
-      unsigned char* sC = pass == 0 ? tile_k(s) : pass == 1 ? tile_q(s) : tile_o(s);
-      unsigned char* sOut = pass == 0 ? tile_q(s) : pass == 1 ? tile_k(s) : tile_v(s);
-      wait(&bar_full[s], n);  // (tiles are read row by row below: every reader has to see the loads' completion itself)
-      wait(&bar_ready[s], n);
-      if (issuer) {
-        if (elect_one() && !*abort_flag) {
-          tc_fence_after_sync();
-          const uint64_t dA = kdesc(smem_u32(sA)), dB = kdesc(smem_u32(sB));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ss(tP, dA + 2 * k, dB + 2 * k, kIdescP, k > 0);
-          mma_commit(&bar_score[pass][s]);
-          if (n > 0) {  // the store of the chunk before: its stage is free when it has been read
-            tma_store_wait_read<0>();
-            mbar_arrive(&bar_free[s ^ 1]);
-          }
-        }
-        __syncwarp();
-      }
+      BwdInfo& f = info[s];
+      unsigned char* sOut = tile_out(s, pass);
+      // (tiles are read row by row below: every reader has to see the loads' completion itself)
+      if (!wait4(&bar_full[s], &bar_ready[s], &bar_score[pass][s], &bar_score[pass][s], n)) break;
+      tc_fence_after_sync();
       const float Gr = f.G[row];
       const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
-      const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
       const float* col = lower ? f.low[wq] : f.up[wq];
-      wait(&bar_score[pass][s], n);
-      tc_fence_after_sync();
       // decayed, masked, packed in place: the half's first 32 columns into its first 16, then the others into the next 16
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
@@ -1305,119 +1368,68 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         tmem_st_x16(tMine + 16 * i, pk);
       }
       tmem_st_wait();
-      sync();
+      tc_fence_before_sync();
+      warp_arrive(&bar_packed[pass], lane);
       float across = 0.f;
-      if (with_state) {  // the state's part, into the accumulator, and scaled there
-        if (issuer) {
-          if (elect_one() && !*abort_flag) {
-            tc_fence_after_sync();
-            const uint64_t dA = kdesc(smem_u32(sA));
-            unsigned char* st = lower ? state_s(s) : state_r(s);
-            if (pass == 2) {  // columns 32 hh .. of R: 64 bytes into its rows
-              const uint64_t d = mdesc(smem_u32(st));
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 4 * hh + 128 * k, kIdescM, k > 0);
-            } else {  // rows 32 hh .. of S, R
-              const uint64_t d = kdesc(smem_u32(st));
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 256 * hh + 2 * k, kIdescK, k > 0);
-            }
-            mma_commit(&bar_state[pass][s]);
-          }
-          __syncwarp();
-        }
-        wait(&bar_state[pass][s], n);
+      if (with_state) {  // the state's part, scaled where it is
+        const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
+        if (!wait4(&bar_state[pass][s], &bar_state[pass][s], &bar_state[pass][s], &bar_state[pass][s], n)) break;
         tc_fence_after_sync();
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           uint32_t r[16];
           tmem_ld_x16(tMine + 32 + 16 * i, r);
           uint4 u, w;
-          if (pass == 1) u = *tile_piece(tile_k(s), row, 4 * half + 2 * i), w = *tile_piece(tile_k(s), row, 4 * half + 2 * i + 1);
+          if (pass == 1) u = *tile_piece(sOut, row, 4 * half + 2 * i), w = *tile_piece(sOut, row, 4 * half + 2 * i + 1);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
-          if (pass == 1) across += dot16<T>(r, u, w);
+          if (pass == 1) across += dot16<T>(r, u, w);  // (dk: the rows of K, over which dk will be written)
           tmem_st_x16(tMine + 32 + 16 * i, r);
         }
         tmem_st_wait();
-        sync();
-      } else if (issuer) {  // (the barrier has one phase per chunk, whether there is a state or not)
-        if (elect_one()) mbar_arrive(&bar_state[pass][s]);
-        __syncwarp();
+        tc_fence_before_sync();
       }
-      if (issuer) {
-        if (elect_one() && !*abort_flag) {
-          tc_fence_after_sync();
-          const uint64_t d = mdesc(smem_u32(sC));
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tP + 64 * hh + 32, tP + 8 * (k & 3) + 64 * (k >> 2), d + 4 * hh + 128 * k, kIdescM, k > 0 || with_state ? 1u : 0u);
-          mma_commit(&bar_rows[pass][s]);
-        }
-        __syncwarp();
-      }
-      wait(&bar_rows[pass][s], n);
-      // the other groups' MMAs that read the tile under the result
-      if (pass == 0) {
-        wait(&bar_score[2][s], n);
-        wait(&bar_rows[1][s], n);
-      } else if (pass == 1) {
-        wait(&bar_score[2][s], n);
-        wait(&bar_rows[0][s], n);
-        if (with_state) wait(&bar_state[2][s], n);
-      } else {
-        wait(&bar_score[0][s], n);
-        wait(&bar_score[1][s], n);
-        if (with_state) wait(&bar_state[1][s], n);
-      }
+      warp_arrive(&bar_scaled[pass], lane);
+      // the rows, and the other groups' MMAs that read the tile under the result
+      if (!(pass == 0   ? wait4(&bar_rows[0][s], &bar_score[2][s], &bar_rows[1][s], &bar_rows[1][s], n)
+            : pass == 1 ? wait4(&bar_rows[1][s], &bar_score[2][s], &bar_rows[0][s], &bar_state[2][s], n)
+                        : wait4(&bar_rows[2][s], &bar_score[0][s], &bar_score[1][s], &bar_state[1][s], n)))
+        break;
       tc_fence_after_sync();
+      uint32_t r[32];
+      tmem_ld_x32(tMine + 32, r);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(&bar_read[pass], lane);
       float dot = 0.f;  // q.dq, k.dk over the half's columns; the result's row takes the place of q's, k's
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t r[16];
-        tmem_ld_x16(tMine + 32 + 16 * i, r);
         uint4 *p0 = tile_piece(sOut, row, 4 * half + 2 * i), *p1 = tile_piece(sOut, row, 4 * half + 2 * i + 1);
+        const uint32_t* x = r + 16 * i;
         uint4 u, w;
-        if (pass < 2) u = *p0, w = *p1;
-        tmem_ld_wait();
-        if (pass < 2) dot += dot16<T>(r, u, w);
-        u.x = Pack2<T>::pack(__uint_as_float(r[0]), __uint_as_float(r[1])), u.y = Pack2<T>::pack(__uint_as_float(r[2]), __uint_as_float(r[3]));
-        u.z = Pack2<T>::pack(__uint_as_float(r[4]), __uint_as_float(r[5])), u.w = Pack2<T>::pack(__uint_as_float(r[6]), __uint_as_float(r[7]));
-        w.x = Pack2<T>::pack(__uint_as_float(r[8]), __uint_as_float(r[9])), w.y = Pack2<T>::pack(__uint_as_float(r[10]), __uint_as_float(r[11]));
-        w.z = Pack2<T>::pack(__uint_as_float(r[12]), __uint_as_float(r[13])), w.w = Pack2<T>::pack(__uint_as_float(r[14]), __uint_as_float(r[15]));
+        if (pass < 2) {
+          u = *p0, w = *p1;
+          dot += dot16<T>(x, u, w);
+        }
+        u.x = Pack2<T>::pack(__uint_as_float(x[0]), __uint_as_float(x[1])), u.y = Pack2<T>::pack(__uint_as_float(x[2]), __uint_as_float(x[3]));
+        u.z = Pack2<T>::pack(__uint_as_float(x[4]), __uint_as_float(x[5])), u.w = Pack2<T>::pack(__uint_as_float(x[6]), __uint_as_float(x[7]));
+        w.x = Pack2<T>::pack(__uint_as_float(x[8]), __uint_as_float(x[9])), w.y = Pack2<T>::pack(__uint_as_float(x[10]), __uint_as_float(x[11]));
+        w.z = Pack2<T>::pack(__uint_as_float(x[12]), __uint_as_float(x[13])), w.w = Pack2<T>::pack(__uint_as_float(x[14]), __uint_as_float(x[15]));
         *p0 = u;
         *p1 = w;
       }
+      fence_proxy_async_smem();
+      warp_arrive(&bar_staged[pass], lane);
       if (pass < 2) {
         if (pass == 0) {
-          info[s].qd[half][row] = dot;
+          f.qd[half][row] = dot;
         } else {
-          info[s].kd[half][row] = dot - across;
-          info[s].bd[half][row] = across;
+          f.kd[half][row] = dot - across;
+          f.bd[half][row] = across;
         }
         warp_arrive(&bar_dots[s], lane);
       }
-      fence_proxy_async_smem();
-      sync();
-      if (issuer) {
-        if (elect_one() && !*abort_flag) {
-          const long bh = unit / a.nchunks;
-          tma_store_tile(pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv, sOut, chunk * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
-          tma_store_commit();
-        }
-        __syncwarp();
-      }
-    }
-    if (issuer) {
-      if (elect_one()) tma_store_wait_read<0>();
-      __syncwarp();
     }
   }
 
