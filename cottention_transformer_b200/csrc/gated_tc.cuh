@@ -1031,13 +1031,14 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
 // and has its half of the accumulator beside it, so that a warp reads what it alone has written over; everything a group does per
 // chunk is a handful of rolled loops that all three run (the one-chunk kernel spent a quarter of its time waiting for instructions
 // and another at its barriers):
-//     scores (MMA) -> decay, pack -> state's part (MMA) -> scale -> rows (MMA) -> result over a tile -> TMA
+//     scores, state's part (MMA) -> decay, pack -> rows (MMA) -> rows + scaled state's part -> result over a tile -> TMA
+// dv has no room in TMEM for a second accumulator: its state's part goes where its rows will be added, and is scaled there first.
 //   warps 0-7: dq over Q     8-15: dk over K     16-23: dv over V     (rows and TMEM lanes 32 (w % 4) .., half (w / 4) % 2)
 //   warps 24-27: gates of the next chunk, masked rows, <S, R>, dg     warp 28: TMA loads
 //   warps 29-31, one thread each: the MMAs and the stores of a pass, so that the scores of the next chunk are under way while the
 //   last rows of this one are written, and no working warp spends its time on issuing
 // Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and
-// 32 of the accumulator.
+// 32 of the accumulator; 64 each for the state's part of dq and dk.
 // A result is staged over a tile when the MMAs that read it have completed, whichever group issued them; the barriers for that are
 // kept per stage, so that nobody can be a whole phase ahead of one that is still waiting.
 // Every wait is bounded.  After one that gave up every further wait returns at once; the warps that share a named barrier go through
@@ -1046,7 +1047,7 @@ constexpr int kBwd64Threads = 1024;
 constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
 constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
 
-struct __align__(16) BwdInfo {  // of a stage's chunk
+struct __align__(16) BwdInfo {  // of a chunk: one more than there are stages, so that a chunk's is made before its tiles arrive
   float G[kGtChunk], low[4][kGtChunk], up[4][kGtChunk];
   float gate[kGtChunk], qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];  // (the dot products by halves)
 };
@@ -1059,9 +1060,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   constexpr bool BF = Pack2<T>::kBf16;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ BwdInfo info[2];
+  __shared__ BwdInfo info[3];
   __shared__ uint64_t bar_full[2], bar_free[2], bar_ready[2], bar_dots[2], bar_score[3][2], bar_state[3][2], bar_rows[3][2];
-  __shared__ uint64_t bar_packed[3], bar_scaled[3], bar_read[3], bar_staged[3];  // a group to its issuing thread, once per chunk each
+  __shared__ uint64_t bar_packed[3], bar_scaled, bar_read[3], bar_staged[3];  // a group to its issuing thread, once per chunk each
   __shared__ uint32_t tmem_slot;
   __shared__ float sPart[12];
   __shared__ int abort_flag_s, loads_s;
@@ -1091,9 +1092,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         mbar_init(&bar_rows[p][s], 1);
       }
     }
+    mbar_init(&bar_scaled, 8);
     for (int p = 0; p < 3; ++p) {
       mbar_init(&bar_packed[p], 8);
-      mbar_init(&bar_scaled[p], 8);
       mbar_init(&bar_read[p], 8);
       mbar_init(&bar_staged[p], 8);
     }
@@ -1127,7 +1128,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     // ---------------------------------------------------------------- MMAs and stores of a pass
     const int pass = warp - 29;
     if (elect_one()) {
-      constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 32, BF, false, false),
+      constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, 64, BF, false, false),
                          kIdescM = make_idesc(128, 32, BF, false, true);
       const uint32_t tP = tmem + 128 * pass;
       const CUtensorMap* out = pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv;
@@ -1152,35 +1153,40 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_ss(tP, dA + 2 * k, dB + 2 * k, kIdescP, k > 0);
         mma_commit(&bar_score[pass][s]);
+        if (pass < 2) {
+          if (with_state) {
+            const uint64_t d = kdesc(smem_u32(pass == 0 ? state_s(s) : state_r(s)));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_ss(tmem + 384 + 64 * pass, dA + 2 * k, d + 2 * k, kIdescK, k > 0);
+            mma_commit(&bar_state[pass][s]);
+          } else {
+            mbar_arrive(&bar_state[pass][s]);  // (one phase per chunk, whether there is a state or not; bar_scaled likewise)
+          }
+        }
         if (n > 0 && !(ok = store(unit - gridDim.x, n - 1))) break;
         if (!(ok = wait_bar1(&bar_packed[pass], n & 1, abort_flag, kWaitScoreReady, n))) break;
-        if (with_state) {  // the state's part, into the accumulator
-          tc_fence_after_sync();
-          if (pass == 2) {  // columns 32 hh .. of R: 64 bytes into its rows
+        tc_fence_after_sync();
+        if (pass == 2) {
+          if (with_state) {  // columns 32 hh .. of R: 64 bytes into its rows
             const uint64_t d = mdesc(smem_u32(state_r(s)));
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
               for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 4 * hh + 128 * k, kIdescM, k > 0);
-          } else {  // rows 32 hh .. of S, R
-            const uint64_t d = kdesc(smem_u32(pass == 0 ? state_s(s) : state_r(s)));
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 256 * hh + 2 * k, kIdescK, k > 0);
+            mma_commit(&bar_state[2][s]);
+          } else {
+            mbar_arrive(&bar_state[2][s]);
           }
-          mma_commit(&bar_state[pass][s]);
-        } else {
-          mbar_arrive(&bar_state[pass][s]);  // (one phase per chunk, whether there is a state or not; bar_scaled likewise)
+          if (!(ok = wait_bar1(&bar_scaled, n & 1, abort_flag, kWaitScoreReady, n))) break;
+          tc_fence_after_sync();
         }
-        if (!(ok = wait_bar1(&bar_scaled[pass], n & 1, abort_flag, kWaitScoreReady, n))) break;
-        tc_fence_after_sync();
+        const bool onto = pass == 2 && with_state;  // the rows are added to what is there
         const uint64_t d = mdesc(smem_u32(tile_c(s, pass)));
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            mma_ts(tP + 64 * hh + 32, tP + 8 * (k & 3) + 64 * (k >> 2), d + 4 * hh + 128 * k, kIdescM, k > 0 || with_state ? 1u : 0u);
+            mma_ts(tP + 64 * hh + 32, tP + 8 * (k & 3) + 64 * (k >> 2), d + 4 * hh + 128 * k, kIdescM, k > 0 || onto ? 1u : 0u);
         mma_commit(&bar_rows[pass][s]);
       }
       if (ok && n > 0) store(unit - gridDim.x, n - 1);
@@ -1217,9 +1223,26 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       for (int e = 0; e < 4; ++e) raw[e] = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
       own = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + t);
     };
-    // dg of the chunk before (unit u, the n-th of this CTA): its dot products, <S, R> as this warp's part
+    // the sums of a chunk's gates and the column factors, from what was fetched
+    auto make_tables = [&](int n) {
+      BwdInfo& f = info[n % 3];
+      named_sync(4, 128);  // (nobody reads what stands there any more)
+      float g[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] = gate_of<T>(raw[e], a.gate_f32);
+      gate_sums<false>(g, lane);
+      if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
+      f.gate[t] = gate_of<T>(own, a.gate_f32);
+      named_sync(4, 128);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        col_factor<true>(f.low, f.G, w, t);
+        col_factor<false>(f.up, f.G, w, t);
+      }
+    };
+    // dg of a chunk that is done (unit u, the n-th of this CTA): its dot products, <S, R> as this warp's part
     auto write_dgate = [&](long u, int n, float cross, bool kept) {
-      const BwdInfo& f = info[n & 1];
+      const BwdInfo& f = info[n % 3];
       wait_bar_warp(&bar_dots[n & 1], (n >> 1) & 1, abort_flag, kWaitAcc, n);
       const long bh = u / a.nchunks, b = bh / a.H;
       const int chunk = static_cast<int>(u % a.nchunks), h = static_cast<int>(bh % a.H), pos = chunk * kGtChunk + t;
@@ -1249,26 +1272,16 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     };
     int n = 0;
     long unit = blockIdx.x;
-    if (unit < a.units) fetch(unit);
+    bool kept = false;
+    if (unit < a.units) {
+      fetch(unit);
+      make_tables(0);
+      kept = own.take != 0;
+      if (unit + gridDim.x < a.units) fetch(unit + gridDim.x);
+    }
     for (; unit < a.units; unit += gridDim.x, ++n) {
       const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
-      const bool kept = own.take != 0;
-      const float gate = gate_of<T>(own, a.gate_f32);
-      float g[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) g[e] = gate_of<T>(raw[e], a.gate_f32);
-      gate_sums<false>(g, lane);
-      wait_bar_warp(&bar_full[s], (n >> 1) & 1, abort_flag, kWaitChunkTma, n);  // (and nobody uses the stage's tables any more)
-      BwdInfo& f = info[s];
-      if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
-      f.gate[t] = gate;
-      if (unit + gridDim.x < a.units) fetch(unit + gridDim.x);
-      named_sync(4, 128);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        col_factor<true>(f.low, f.G, w, t);
-        col_factor<false>(f.up, f.G, w, t);
-      }
+      wait_bar_warp(&bar_full[s], (n >> 1) & 1, abort_flag, kWaitChunkTma, n);
       if (a.keep) {  // nothing of a masked position gets into a product
         if (!kept) {
           const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -1295,9 +1308,16 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         for (int off = 16; off > 0; off >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, off);
       }
       warp_arrive(&bar_free[s], lane);
+      // the next chunk's tables, where those of two chunks ago were: the tiles that have just arrived are in the stage that it left
+      const bool kept_now = kept;
+      if (unit + gridDim.x < a.units) {
+        make_tables(n + 1);
+        kept = own.take != 0;
+        if (unit + 2 * static_cast<long>(gridDim.x) < a.units) fetch(unit + 2 * static_cast<long>(gridDim.x));
+      }
       if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
       cross_before = cross;
-      kp_before = kept;
+      kp_before = kept_now;
     }
     if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
   } else {
@@ -1306,6 +1326,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     const bool lower = pass == 0;
     const uint32_t tMine = tmem + 128 * pass + 64 * half + lane_base;
     const float sign = lower ? 1.f : -1.f;
+    const uint32_t tState = tmem + 384 + 64 * pass + 32 * half + lane_base;
     const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
     // up to four barriers at once: one round trip
     auto wait4 = [&](uint64_t* b0, uint64_t* b1, uint64_t* b2, uint64_t* b3, int n) {
@@ -1323,12 +1344,12 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
       const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
       const bool with_state = lower ? has_s(chunk) : has_r(chunk);
-      BwdInfo& f = info[s];
+      BwdInfo& f = info[n % 3];
       unsigned char* sOut = tile_out(s, pass);
       // (tiles are read row by row below: every reader has to see the loads' completion itself)
       if (!wait4(&bar_full[s], &bar_ready[s], &bar_score[pass][s], &bar_score[pass][s], n)) break;
       tc_fence_after_sync();
-      const float Gr = f.G[row];
+      const float Gr = f.G[row], signedG = sign * Gr;
       const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
       const float* col = lower ? f.low[wq] : f.up[wq];
       // decayed, masked, packed in place: the half's first 32 columns into its first 16, then the others into the next 16
@@ -1350,7 +1371,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
               const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
               float x[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * ex2(sign * (Gr - gs[e])) : 0.f;
+              for (int e = 0; e < 4; ++e) x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * ex2(fmaf(-sign, gs[e], signedG)) : 0.f;
               pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
               pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
             }
@@ -1370,47 +1391,56 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       tmem_st_wait();
       tc_fence_before_sync();
       warp_arrive(&bar_packed[pass], lane);
-      float across = 0.f;
-      if (with_state) {  // the state's part, scaled where it is
-        const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
-        if (!wait4(&bar_state[pass][s], &bar_state[pass][s], &bar_state[pass][s], &bar_state[pass][s], n)) break;
-        tc_fence_after_sync();
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          uint32_t r[16];
-          tmem_ld_x16(tMine + 32 + 16 * i, r);
-          uint4 u, w;
-          if (pass == 1) u = *tile_piece(sOut, row, 4 * half + 2 * i), w = *tile_piece(sOut, row, 4 * half + 2 * i + 1);
+      const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
+      if (pass == 2) {
+        if (with_state) {  // dv: the state's part, scaled where it is
+          if (!wait4(&bar_state[2][s], &bar_state[2][s], &bar_state[2][s], &bar_state[2][s], n)) break;
+          tc_fence_after_sync();
+          uint32_t r[32];
+          tmem_ld_x32(tMine + 32, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
-          if (pass == 1) across += dot16<T>(r, u, w);  // (dk: the rows of K, over which dk will be written)
-          tmem_st_x16(tMine + 32 + 16 * i, r);
+          for (int j = 0; j < 32; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
+          tmem_st_x32(tMine + 32, r);
+          tmem_st_wait();
+          tc_fence_before_sync();
         }
-        tmem_st_wait();
-        tc_fence_before_sync();
+        warp_arrive(&bar_scaled, lane);
       }
-      warp_arrive(&bar_scaled[pass], lane);
       // the rows, and the other groups' MMAs that read the tile under the result
       if (!(pass == 0   ? wait4(&bar_rows[0][s], &bar_score[2][s], &bar_rows[1][s], &bar_rows[1][s], n)
             : pass == 1 ? wait4(&bar_rows[1][s], &bar_score[2][s], &bar_rows[0][s], &bar_state[2][s], n)
                         : wait4(&bar_rows[2][s], &bar_score[0][s], &bar_score[1][s], &bar_state[1][s], n)))
         break;
       tc_fence_after_sync();
-      uint32_t r[32];
-      tmem_ld_x32(tMine + 32, r);
-      tmem_ld_wait();
-      tc_fence_before_sync();
-      warp_arrive(&bar_read[pass], lane);
-      float dot = 0.f;  // q.dq, k.dk over the half's columns; the result's row takes the place of q's, k's
-#pragma unroll
+      float dot = 0.f, across = 0.f;  // q.dq, k.dk over the half's columns; the result's row takes the place of q's, k's
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         uint4 *p0 = tile_piece(sOut, row, 4 * half + 2 * i), *p1 = tile_piece(sOut, row, 4 * half + 2 * i + 1);
-        const uint32_t* x = r + 16 * i;
+        uint32_t x[16];
+        tmem_ld_x16(tMine + 32 + 16 * i, x);
         uint4 u, w;
         if (pass < 2) {
           u = *p0, w = *p1;
+          if (with_state) {
+            uint32_t y[16];
+            tmem_ld_x16(tState + 16 * i, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(y[j]));
+            if (pass == 1) across += dot16<T>(y, u, w);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) + __uint_as_float(y[j]));
+          } else {
+            tmem_ld_wait();
+          }
           dot += dot16<T>(x, u, w);
+        } else {
+          tmem_ld_wait();
+        }
+        if (i == 1) {
+          tc_fence_before_sync();
+          warp_arrive(&bar_read[pass], lane);
         }
         u.x = Pack2<T>::pack(__uint_as_float(x[0]), __uint_as_float(x[1])), u.y = Pack2<T>::pack(__uint_as_float(x[2]), __uint_as_float(x[3]));
         u.z = Pack2<T>::pack(__uint_as_float(x[4]), __uint_as_float(x[5])), u.w = Pack2<T>::pack(__uint_as_float(x[6]), __uint_as_float(x[7]));
