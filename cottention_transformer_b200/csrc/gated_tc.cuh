@@ -473,12 +473,28 @@ template <bool LOWER>
 __device__ __forceinline__ void col_factor(float (*sCol)[kGtChunk], const float* sG, int w, int s) {
   if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = ex2(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {  // two products in one instruction
+// Two products, two multiply-adds in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 c;
   asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
       : "=f"(c.x), "=f"(c.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair(const uint32_t* r) { return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+// acc += 16 values times two packed pieces of a row
+template <typename T>
+__device__ __forceinline__ void dot16_2(float2& acc, const uint32_t* x, const uint4& u, const uint4& w) {
+  const uint32_t p[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc = fma2(Pack2<T>::unpack(p[j]), pair(x + 2 * j), acc);
 }
 // 32 columns (block `blk`) of the scores of a row of block wq, decayed, masked and packed
 template <typename T, bool LOWER>
@@ -1049,6 +1065,7 @@ constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
 
 struct __align__(16) BwdInfo {  // of a chunk: one more than there are stages, so that a chunk's is made before its tiles arrive
   float G[kGtChunk], low[4][kGtChunk], up[4][kGtChunk];
+  int has_s, has_r;
   float gate[kGtChunk], qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];  // (the dot products by halves)
 };
 
@@ -1224,7 +1241,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       own = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + t);
     };
     // the sums of a chunk's gates and the column factors, from what was fetched
-    auto make_tables = [&](int n) {
+    auto make_tables = [&](int n, int chunk) {
       BwdInfo& f = info[n % 3];
       named_sync(4, 128);  // (nobody reads what stands there any more)
       float g[4];
@@ -1233,6 +1250,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       gate_sums<false>(g, lane);
       if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
       f.gate[t] = gate_of<T>(own, a.gate_f32);
+      if (t == 0) f.has_s = has_s(chunk), f.has_r = has_r(chunk);
       named_sync(4, 128);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -1275,7 +1293,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     bool kept = false;
     if (unit < a.units) {
       fetch(unit);
-      make_tables(0);
+      make_tables(0, static_cast<int>(unit % a.nchunks));
       kept = own.take != 0;
       if (unit + gridDim.x < a.units) fetch(unit + gridDim.x);
     }
@@ -1311,7 +1329,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       // the next chunk's tables, where those of two chunks ago were: the tiles that have just arrived are in the stage that it left
       const bool kept_now = kept;
       if (unit + gridDim.x < a.units) {
-        make_tables(n + 1);
+        make_tables(n + 1, static_cast<int>((unit + gridDim.x) % a.nchunks));
         kept = own.take != 0;
         if (unit + 2 * static_cast<long>(gridDim.x) < a.units) fetch(unit + 2 * static_cast<long>(gridDim.x));
       }
@@ -1328,12 +1346,13 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     const float sign = lower ? 1.f : -1.f;
     const uint32_t tState = tmem + 384 + 64 * pass + 32 * half + lane_base;
     const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
-    // up to four barriers at once: one round trip
-    auto wait4 = [&](uint64_t* b0, uint64_t* b1, uint64_t* b2, uint64_t* b3, int n) {
+    // several barriers at once: one round trip
+    auto wait = [&](int n, auto... bars) {
       const uint32_t parity = (n >> 1) & 1;
       for (uint32_t i = 0; i < kMaxPolls; ++i) {
-        const bool d0 = mbar_try_wait(b0, parity), d1 = mbar_try_wait(b1, parity), d2 = mbar_try_wait(b2, parity), d3 = mbar_try_wait(b3, parity);
-        if (__all_sync(0xffffffffu, d0 && d1 && d2 && d3)) return true;
+        bool done = true;
+        ((done = mbar_try_wait(bars, parity) && done), ...);
+        if (__all_sync(0xffffffffu, done)) return true;
         if (*abort_flag) return false;
       }
       *abort_flag = 1;
@@ -1342,13 +1361,13 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     };
     int n = 0;
     for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
-      const int s = n & 1, chunk = static_cast<int>(unit % a.nchunks);
-      const bool with_state = lower ? has_s(chunk) : has_r(chunk);
+      const int s = n & 1;
       BwdInfo& f = info[n % 3];
       unsigned char* sOut = tile_out(s, pass);
       // (tiles are read row by row below: every reader has to see the loads' completion itself)
-      if (!wait4(&bar_full[s], &bar_ready[s], &bar_score[pass][s], &bar_score[pass][s], n)) break;
+      if (!wait(n, &bar_full[s], &bar_ready[s], &bar_score[pass][s])) break;
       tc_fence_after_sync();
+      const bool with_state = lower ? f.has_s : f.has_r;
       const float Gr = f.G[row], signedG = sign * Gr;
       const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
       const float* col = lower ? f.low[wq] : f.up[wq];
@@ -1368,19 +1387,21 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 Gs = *reinterpret_cast<const float4*>(&f.G[32 * blk + j]);
-              const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
-              float x[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = keep_bits & (1u << (j + e)) ? __uint_as_float(r[j + e]) * ex2(fmaf(-sign, gs[e], signedG)) : 0.f;
-              pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
-              pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
+              for (int e = 0; e < 4; e += 2) {
+                float2 x = fma2(make_float2(-sign, -sign), e ? make_float2(Gs.z, Gs.w) : make_float2(Gs.x, Gs.y), make_float2(signedG, signedG));
+                x = mul2(make_float2(ex2(x.x), ex2(x.y)), pair(r + j + e));
+                x.x = keep_bits & (1u << (j + e)) ? x.x : 0.f;
+                x.y = keep_bits & (2u << (j + e)) ? x.y : 0.f;
+                pk[(j + e) / 2] = Pack2<T>::pack(x.x, x.y);
+              }
             }
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 cf = *reinterpret_cast<const float4*>(&col[32 * blk + j]);
-              const float2 x = mul2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2(make_float2(cf.x, cf.y), make_float2(rowf, rowf)));
-              const float2 y = mul2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), mul2(make_float2(cf.z, cf.w), make_float2(rowf, rowf)));
+              const float2 x = mul2(pair(r + j), mul2(make_float2(cf.x, cf.y), make_float2(rowf, rowf)));
+              const float2 y = mul2(pair(r + j + 2), mul2(make_float2(cf.z, cf.w), make_float2(rowf, rowf)));
               pk[j / 2] = Pack2<T>::pack(x.x, x.y);
               pk[j / 2 + 1] = Pack2<T>::pack(y.x, y.y);
             }
@@ -1394,13 +1415,16 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
       if (pass == 2) {
         if (with_state) {  // dv: the state's part, scaled where it is
-          if (!wait4(&bar_state[2][s], &bar_state[2][s], &bar_state[2][s], &bar_state[2][s], n)) break;
+          if (!wait(n, &bar_state[2][s])) break;
           tc_fence_after_sync();
           uint32_t r[32];
           tmem_ld_x32(tMine + 32, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(r[j]));
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = mul2(pair(r + j), make_float2(scale, scale));
+            r[j] = __float_as_uint(x.x), r[j + 1] = __float_as_uint(x.y);
+          }
           tmem_st_x32(tMine + 32, r);
           tmem_st_wait();
           tc_fence_before_sync();
@@ -1408,12 +1432,13 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         warp_arrive(&bar_scaled, lane);
       }
       // the rows, and the other groups' MMAs that read the tile under the result
-      if (!(pass == 0   ? wait4(&bar_rows[0][s], &bar_score[2][s], &bar_rows[1][s], &bar_rows[1][s], n)
-            : pass == 1 ? wait4(&bar_rows[1][s], &bar_score[2][s], &bar_rows[0][s], &bar_state[2][s], n)
-                        : wait4(&bar_rows[2][s], &bar_score[0][s], &bar_score[1][s], &bar_state[1][s], n)))
+      if (!(pass == 0   ? wait(n, &bar_rows[0][s], &bar_score[2][s], &bar_rows[1][s])
+            : pass == 1 ? wait(n, &bar_rows[1][s], &bar_score[2][s], &bar_rows[0][s], &bar_state[2][s])
+                        : wait(n, &bar_rows[2][s], &bar_score[0][s], &bar_score[1][s], &bar_state[1][s])))
         break;
       tc_fence_after_sync();
-      float dot = 0.f, across = 0.f;  // q.dq, k.dk over the half's columns; the result's row takes the place of q's, k's
+      // q.dq, k.dk over the half's columns (k.dk by parts); the result's row takes the place of q's, k's
+      float2 dot = make_float2(0.f, 0.f), across = make_float2(0.f, 0.f);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         uint4 *p0 = tile_piece(sOut, row, 4 * half + 2 * i), *p1 = tile_piece(sOut, row, 4 * half + 2 * i + 1);
@@ -1422,19 +1447,19 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         uint4 u, w;
         if (pass < 2) {
           u = *p0, w = *p1;
+          uint32_t y[16];
+          if (with_state) tmem_ld_x16(tState + 16 * i, y);
+          tmem_ld_wait();
+          if (pass == 1) dot16_2<T>(dot, x, u, w);
           if (with_state) {
-            uint32_t y[16];
-            tmem_ld_x16(tState + 16 * i, y);
-            tmem_ld_wait();
+            if (pass == 1) dot16_2<T>(across, y, u, w);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = scale == 0.f ? 0u : __float_as_uint(scale * __uint_as_float(y[j]));
-            if (pass == 1) across += dot16<T>(y, u, w);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) + __uint_as_float(y[j]));
-          } else {
-            tmem_ld_wait();
+            for (int j = 0; j < 16; j += 2) {
+              const float2 z = fma2(pair(y + j), make_float2(scale, scale), pair(x + j));
+              x[j] = __float_as_uint(z.x), x[j + 1] = __float_as_uint(z.y);
+            }
           }
-          dot += dot16<T>(x, u, w);
+          if (pass == 0) dot16_2<T>(dot, x, u, w);
         } else {
           tmem_ld_wait();
         }
@@ -1453,10 +1478,10 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       warp_arrive(&bar_staged[pass], lane);
       if (pass < 2) {
         if (pass == 0) {
-          f.qd[half][row] = dot;
+          f.qd[half][row] = dot.x + dot.y;
         } else {
-          f.kd[half][row] = dot - across;
-          f.bd[half][row] = across;
+          f.kd[half][row] = dot.x + dot.y;
+          f.bd[half][row] = scale * (across.x + across.y);
         }
         warp_arrive(&bar_dots[s], lane);
       }
