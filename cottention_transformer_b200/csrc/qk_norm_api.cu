@@ -24,11 +24,29 @@ template <typename T> struct Piece {
   __device__ __forceinline__ Piece() {}
 };
 
+// Division of numbers below 2^31 by a number known at launch: m = ceil(2^(31+s) / d) with 2^s >= d has d m - 2^(31+s) < 2^s, which
+// is what makes (r m) >> (31+s) exact.  (Two divisions per row are otherwise most of a row's instructions.)
+struct Divider {
+  unsigned d, m;
+  int shift;
+};
+Divider divider(unsigned d) {
+  Divider r = {d, 0, 31};
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  r.shift = 31 + s;
+  r.m = (unsigned)(((1ull << r.shift) + d - 1) / d);
+  return r;
+}
+__device__ __forceinline__ unsigned divide(unsigned r, const Divider& d) {
+  return static_cast<unsigned>((static_cast<unsigned long long>(r) * d.m) >> d.shift);
+}
+
 struct NormSide {  // q or k
   const void *x, *w, *dy;
   void *y, *dx;
   cott_strides sx, sy, sdy, sdx;
-  int H;
+  Divider heads;
   unsigned rows;  // B * N * H
 };
 struct NormArgs {
@@ -36,17 +54,18 @@ struct NormArgs {
   const float *sin_t, *cos_t;
   float* partial;  // backward: [2][CTAs][D]
   long long table_batch_stride;
-  int N, rot, w_f32;
+  Divider positions;
+  int rot, w_f32;
   float eps;
 };
 
 // The row numbered `r` of a side: consecutive numbers walk the heads of a position, then the positions, then the batch.
 struct RowAt {
-  int b, n, h;
+  unsigned b, n, h;
 };
-__device__ __forceinline__ RowAt row_at(unsigned r, int H, int N) {
-  const unsigned p = r / static_cast<unsigned>(H), b = p / static_cast<unsigned>(N);
-  return RowAt{static_cast<int>(b), static_cast<int>(p - b * N), static_cast<int>(r - p * H)};
+__device__ __forceinline__ RowAt row_at(unsigned r, const Divider& heads, const Divider& positions) {
+  const unsigned p = divide(r, heads), b = divide(p, positions);
+  return RowAt{b, p - b * positions.d, r - p * heads.d};
 }
 __device__ __forceinline__ long long at(const cott_strides& s, const RowAt& r) { return r.b * s.b + r.h * s.h + r.n * s.n; }
 
@@ -81,42 +100,49 @@ __device__ __forceinline__ void rotate(float (&x)[E], const float* sin_t, const 
   }
 }
 
-// grid = (CTAs, 2): y = q, k.  Each CTA takes every gridDim.x-th group of rows.
-template <typename T, int D>
+// grid = (CTAs, 2): y = q, k.  A CTA takes U groups of rows at a time, all of whose loads are in flight together: with one group
+// the pass reached 3.6 TB/s.
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_fwd_kernel(const NormArgs a) {
-  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;  // elements and lanes of a piece, rows per CTA and round
+  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;  // elements and lanes of a piece, rows per group
   const NormSide& s = a.side[blockIdx.y];
   const int piece = threadIdx.x % LPR, c = piece * E;
   pdl_allow_next();
   pdl_wait_prior();
   float w[E];
   load_weights<T, E>(w, s.w, a.w_f32, c);
-  for (unsigned r0 = blockIdx.x * RPC; r0 < s.rows; r0 += gridDim.x * RPC) {
-    const unsigned r = r0 + threadIdx.x / LPR;
-    const bool in = r < s.rows;
-    const RowAt row = row_at(in ? r : s.rows - 1, s.H, a.N);
-    Piece<T> p;
-    p.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row) + c);
-    float x[E], sum = 0.f;
+  for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
+    RowAt row[U];
+    Piece<T> p[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = to_acc(p.e[e]);
-      sum = fmaf(x[e], x[e], sum);
-    }
-    const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * rms * w[e];
-    if (c < a.rot) {
-      const long long t = row.b * a.table_batch_stride + static_cast<long long>(row.n) * (a.rot / 2) + c / 2;
-      rotate<E>(x, a.sin_t + t, a.cos_t + t, 1.f);
+    for (int u = 0; u < U; ++u) {
+      const unsigned r = r0 + u * RPC + threadIdx.x / LPR;
+      row[u] = row_at(r < s.rows ? r : s.rows - 1, s.heads, a.positions);
+      p[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row[u]) + c);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) p.e[e] = from_acc<T>(x[e]);
-    if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row) + c) = p.u;
+    for (int u = 0; u < U; ++u) {
+      float x[E], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        x[e] = to_acc(p[u].e[e]);
+        sum = fmaf(x[e], x[e], sum);
+      }
+      const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] * rms * w[e];
+      if (c < a.rot) {
+        const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
+        rotate<E>(x, a.sin_t + t, a.cos_t + t, 1.f);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[u].e[e] = from_acc<T>(x[e]);
+      if (r0 + u * RPC + threadIdx.x / LPR < s.rows) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row[u]) + c) = p[u].u;
+    }
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArgs a) {
   constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;
   const NormSide& s = a.side[blockIdx.y];
@@ -128,37 +154,44 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArg
   load_weights<T, E>(w, s.w, a.w_f32, c);
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = 0.f;
-  for (unsigned r0 = blockIdx.x * RPC; r0 < s.rows; r0 += gridDim.x * RPC) {
-    const unsigned r = r0 + threadIdx.x / LPR;
-    const bool in = r < s.rows;
-    const RowAt row = row_at(in ? r : s.rows - 1, s.H, a.N);
-    Piece<T> p, d;
-    p.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row) + c);
-    d.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.dy) + at(s.sdy, row) + c);
-    float x[E], f[E], sum = 0.f;
+  for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
+    RowAt row[U];
+    Piece<T> p[U], d[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = to_acc(p.e[e]);
-      f[e] = to_acc(d.e[e]);
-      sum = fmaf(x[e], x[e], sum);
+    for (int u = 0; u < U; ++u) {
+      const unsigned r = r0 + u * RPC + threadIdx.x / LPR;
+      row[u] = row_at(r < s.rows ? r : s.rows - 1, s.heads, a.positions);
+      p[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row[u]) + c);
+      d[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.dy) + at(s.sdy, row[u]) + c);
     }
-    if (c < a.rot) {
-      const long long t = row.b * a.table_batch_stride + static_cast<long long>(row.n) * (a.rot / 2) + c / 2;
-      rotate<E>(f, a.sin_t + t, a.cos_t + t, -1.f);
-    }
-    const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
-    float dot = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] *= rms;
-      if (in) dw[e] = fmaf(f[e], x[e], dw[e]);
-      f[e] *= w[e];
-      dot = fmaf(f[e], x[e], dot);
-    }
-    dot = row_sum<LPR>(dot) * (1.f / D);
+    for (int u = 0; u < U; ++u) {
+      const bool in = r0 + u * RPC + threadIdx.x / LPR < s.rows;
+      float x[E], f[E], sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) p.e[e] = from_acc<T>(rms * (f[e] - x[e] * dot));
-    if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row) + c) = p.u;
+      for (int e = 0; e < E; ++e) {
+        x[e] = to_acc(p[u].e[e]);
+        f[e] = to_acc(d[u].e[e]);
+        sum = fmaf(x[e], x[e], sum);
+      }
+      if (c < a.rot) {
+        const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
+        rotate<E>(f, a.sin_t + t, a.cos_t + t, -1.f);
+      }
+      const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        x[e] *= rms;
+        if (in) dw[e] = fmaf(f[e], x[e], dw[e]);
+        f[e] *= w[e];
+        dot = fmaf(f[e], x[e], dot);
+      }
+      dot = row_sum<LPR>(dot) * (1.f / D);
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[u].e[e] = from_acc<T>(rms * (f[e] - x[e] * dot));
+      if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row[u]) + c) = p[u].u;
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) part[threadIdx.x / LPR][c + e] = dw[e];
@@ -171,23 +204,23 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArg
   }
 }
 
-// dw of q and of k: the sums of the CTAs, in their order.  grid = (D / 32, 2), block = 256: 32 columns, eight threads each.
+// dw of q and of k: the sums of the CTAs, in a fixed order.  grid = (D / 32, 2), block = 1024: 32 columns, 32 threads each.
 template <typename T>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_dw_kernel(const float* __restrict__ partial, void* dqw, void* dkw, int ctas, int D, int w_f32) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restrict__ partial, void* dqw, void* dkw, int ctas, int D, int w_f32) {
+  __shared__ float part[32][33];
   const int col = threadIdx.x & 31, u = threadIdx.x >> 5, e = blockIdx.x * 32 + col;
   pdl_allow_next();
   pdl_wait_prior();
   const float* src = partial + static_cast<long>(blockIdx.y) * ctas * D;
   float sum = 0.f;
-#pragma unroll 4
-  for (int i = u; i < ctas; i += 8) sum += src[static_cast<long>(i) * D + e];
+#pragma unroll 8
+  for (int i = u; i < ctas; i += 32) sum += src[static_cast<long>(i) * D + e];
   part[u][col] = sum;
   __syncthreads();
   if (u == 0) {
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += part[i][col];
+    for (int i = 0; i < 32; ++i) sum += part[i][col];
     void* dst = blockIdx.y ? dkw : dqw;
     if (w_f32)
       static_cast<float*>(dst)[e] = sum;
@@ -227,19 +260,23 @@ int norm_ctas(unsigned rows, int rows_per_cta, int resident) {
   const long want = ((long)rows + rows_per_cta - 1) / rows_per_cta, most = (long)sm * resident;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
-constexpr int kBwdResident = 3;
+constexpr int kBwdResident = 4, kFwdGroups = 4, kBwdGroups = 2;
 
 template <typename T, int D>
 int launch_norm(const NormArgs& a, bool bwd, void* dqw, void* dkw, cudaStream_t stream) {
   constexpr int RPC = kNormThreads / (D / Piece<T>::kElems);
   const unsigned rows = a.side[0].rows > a.side[1].rows ? a.side[0].rows : a.side[1].rows;
   if (!bwd) {
-    COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D>, dim3(norm_ctas(rows, RPC, 64), 2), kNormThreads, 0, stream, a));
+    // (few rows, as of new tokens: one group per CTA, so that they are spread over the SMs)
+    if (rows <= 148u * RPC)
+      COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D, 1>, dim3(norm_ctas(rows, RPC, 64), 2), kNormThreads, 0, stream, a));
+    else
+      COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D, kFwdGroups>, dim3(norm_ctas(rows, RPC * kFwdGroups, 64), 2), kNormThreads, 0, stream, a));
     return COTT_OK;
   }
-  const int ctas = norm_ctas(rows, RPC, kBwdResident);
-  COTT_CUDA_TRY(launch_pdl(qk_norm_bwd_kernel<T, D>, dim3(ctas, 2), kNormThreads, 0, stream, a));
-  COTT_CUDA_TRY(launch_pdl(qk_norm_dw_kernel<T>, dim3(D / 32, 2), kNormThreads, 0, stream, static_cast<const float*>(a.partial), dqw, dkw, ctas, D, a.w_f32));
+  const int ctas = norm_ctas(rows, RPC * kBwdGroups, kBwdResident);
+  COTT_CUDA_TRY(launch_pdl(qk_norm_bwd_kernel<T, D, kBwdGroups>, dim3(ctas, 2), kNormThreads, 0, stream, a));
+  COTT_CUDA_TRY(launch_pdl(qk_norm_dw_kernel<T>, dim3(D / 32, 2), 1024, 0, stream, static_cast<const float*>(a.partial), dqw, dkw, ctas, D, a.w_f32));
   return COTT_OK;
 }
 template <typename T>
@@ -261,11 +298,11 @@ NormArgs norm_args(const cott_norm_layout* l, const void* q, const void* k, cons
                    int Hq, int Hk, int N, int D, int weight_dtype, float eps) {
   NormArgs a = {};
   const cott_strides dq = {(long long)Hq * N * D, (long long)N * D, D}, dk = {(long long)Hk * N * D, (long long)N * D, D};
-  a.side[0].x = q, a.side[0].w = qw, a.side[0].H = Hq, a.side[0].rows = (unsigned)((long)B * N * Hq), a.side[0].sx = l ? l->q : dq;
-  a.side[1].x = k, a.side[1].w = kw, a.side[1].H = Hk, a.side[1].rows = (unsigned)((long)B * N * Hk), a.side[1].sx = l ? l->k : dk;
+  a.side[0].x = q, a.side[0].w = qw, a.side[0].heads = divider(Hq), a.side[0].rows = (unsigned)((long)B * N * Hq), a.side[0].sx = l ? l->q : dq;
+  a.side[1].x = k, a.side[1].w = kw, a.side[1].heads = divider(Hk), a.side[1].rows = (unsigned)((long)B * N * Hk), a.side[1].sx = l ? l->k : dk;
   a.side[0].sy = a.side[0].sdy = l ? l->q_out : dq, a.side[1].sy = a.side[1].sdy = l ? l->k_out : dk;
   a.side[0].sdx = l ? l->dq : dq, a.side[1].sdx = l ? l->dk : dk;
-  a.N = N, a.w_f32 = weight_dtype == COTT_F32, a.eps = eps;
+  a.positions = divider(N), a.w_f32 = weight_dtype == COTT_F32, a.eps = eps;
   if (rotary) a.sin_t = rotary->sin_table, a.cos_t = rotary->cos_table, a.rot = rotary->rot_dim, a.table_batch_stride = rotary->table_batch_stride;
   return a;
 }
@@ -279,12 +316,13 @@ int cott_qk_norm_fwd(const void* q, const void* k, const void* q_weight, const v
   int st = check_norm_args(B, Hq, Hk, N, D, dtype, weight_dtype, rotary);
   if (st) return st;
   if ((long)B * N * (Hq + Hk) == 0) return COTT_OK;
+  if (!Hq || !Hk) return fail(COTT_ERR_SHAPE, "q and k need a head each");
   NormArgs a = norm_args(layout, q, k, q_weight, k_weight, rotary, B, Hq, Hk, N, D, weight_dtype, eps);
   a.side[0].y = q_out, a.side[1].y = k_out;
-  if (Hq && ((st = check_norm_rows("q", q, a.side[0].sx, dtype)) || (st = check_norm_rows("q_out", q_out, a.side[0].sy, dtype)))) return st;
-  if (Hk && ((st = check_norm_rows("k", k, a.side[1].sx, dtype)) || (st = check_norm_rows("k_out", k_out, a.side[1].sy, dtype)))) return st;
-  if ((Hq && !q_weight) || (Hk && !k_weight)) return fail(COTT_ERR_NULL, "null pointer: weight");
-  if (!Hq || !Hk) return fail(COTT_ERR_SHAPE, "q and k need a head each");
+  if ((st = check_norm_rows("q", q, a.side[0].sx, dtype)) || (st = check_norm_rows("q_out", q_out, a.side[0].sy, dtype)) ||
+      (st = check_norm_rows("k", k, a.side[1].sx, dtype)) || (st = check_norm_rows("k_out", k_out, a.side[1].sy, dtype)))
+    return st;
+  if (!q_weight || !k_weight) return fail(COTT_ERR_NULL, "null pointer: weight");
   DeviceScope scope(q);
   COTT_CUDA_TRY(scope.status());
   return launch_norm_any(a, D, dtype, false, nullptr, nullptr, static_cast<cudaStream_t>(stream));

@@ -589,29 +589,44 @@ Grads gated_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, c
         "cott_gated_scan_bwd");
   return {dq, dk, dv, dg, dinit};
 }
+struct GatedCall {  // what a forward leaves
+  at::Tensor q, k, v, out, final, states;
+  OptTensor keep;
+  bool with_initial;
+};
+GatedCall gated_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& gate, const OptTensor& keep, const OptTensor& initial,
+                    bool return_state) {
+  GatedCall c;
+  c.q = rows16(q_), c.k = rows16(k_), c.v = rows16(v_);
+  const OptTensor init = has(initial) ? OptTensor(dense16(*initial)) : OptTensor();
+  c.keep = gated_keep(keep, c.q);
+  c.with_initial = has(init);
+  const int B = (int)c.q.size(0), H = (int)c.q.size(1), N = (int)c.q.size(2), D = (int)c.q.size(3), code = dtype_code(c.q.scalar_type());
+  const c10::cuda::CUDAGuard guard(c.q.device());
+  c.out = at::empty_like(c.v);
+  if (return_state) c.final = state_like(c.q);
+  c.states = bytes_like(c.q, cott_gated_scan_states_bytes(B, H, N, D, code));
+  const size_t need = cott_gated_scan_workspace_bytes(B, H, N, D, code, 0);
+  const at::Tensor ws = need ? bytes_like(c.q, need) : at::Tensor();
+  cott_gated_layout lay = {};
+  lay.q = strides3(c.q), lay.k = strides3(c.k), lay.v = strides3(c.v), lay.out = strides3(c.out), lay.gate = strides3(gate);
+  check(cott_gated_scan_fwd(c.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), gate.data_ptr(), u8(c.keep), f32_or_null(init), c.out.data_ptr(),
+                            return_state ? c.final.data_ptr<float>() : nullptr, c.states.data_ptr(), need ? ws.data_ptr() : nullptr, &lay, B, H, N, D, code,
+                            dtype_code(gate.scalar_type()), stream_of(c.q)),
+        "cott_gated_scan_fwd");
+  return c;
+}
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& gate,
                                const OptTensor& keep, const OptTensor& initial, bool return_state, bool want_dinitial) {
-    const at::Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
-    const OptTensor init = has(initial) ? OptTensor(dense16(*initial)) : OptTensor(), kp = gated_keep(keep, q);
-    const int B = (int)q.size(0), H = (int)q.size(1), N = (int)q.size(2), D = (int)q.size(3), code = dtype_code(q.scalar_type());
-    const c10::cuda::CUDAGuard guard(q.device());
-    at::Tensor out = at::empty_like(v), final = return_state ? state_like(q) : at::Tensor();
-    const at::Tensor states = bytes_like(q, cott_gated_scan_states_bytes(B, H, N, D, code)),
-                     ws = bytes_like(q, cott_gated_scan_workspace_bytes(B, H, N, D, code, 0));
-    cott_gated_layout lay = {};
-    lay.q = strides3(q), lay.k = strides3(k), lay.v = strides3(v), lay.out = strides3(out), lay.gate = strides3(gate);
-    check(cott_gated_scan_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), gate.data_ptr(), u8(kp), f32_or_null(init), out.data_ptr(),
-                              return_state ? final.data_ptr<float>() : nullptr, states.data_ptr(), ws.data_ptr(), &lay, B, H, N, D, code,
-                              dtype_code(gate.scalar_type()), stream_of(q)),
-          "cott_gated_scan_fwd");
+    GatedCall c = gated_fwd(q_, k_, v_, gate, keep, initial, return_state);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, gate});
-    ctx->saved_data["states"] = states;
-    ctx->saved_data["with_initial"] = has(init);
+    ctx->save_for_backward({c.q, c.k, c.v, gate});
+    ctx->saved_data["states"] = c.states;
+    ctx->saved_data["with_initial"] = c.with_initial;
     ctx->saved_data["want_dinitial"] = want_dinitial;
-    save_opt(ctx, "keep", kp);
-    return return_state ? variable_list{out, final} : variable_list{out};
+    save_opt(ctx, "keep", c.keep);
+    return return_state ? variable_list{c.out, c.final} : variable_list{c.out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
@@ -634,6 +649,11 @@ variable_list gated_scan(const at::Tensor& q, const at::Tensor& k, const at::Ten
                          const OptTensor& initial, bool return_state) {
   check_gated("gated_scan", q, k, v, log_decay);
   if (has(initial)) check_gated_state("initial_state", *initial, q);
+  if (!at::GradMode::is_enabled() ||
+      !(q.requires_grad() || k.requires_grad() || v.requires_grad() || log_decay.requires_grad() || (has(initial) && initial->requires_grad()))) {
+    GatedCall c = gated_fwd(q, k, v, log_decay, keep, initial, return_state);
+    return return_state ? variable_list{c.out, c.final} : variable_list{c.out};
+  }
   return GatedFn::apply(q, k, v, log_decay, keep, initial, return_state,
                         has(initial) && at::GradMode::is_enabled() && initial->requires_grad());
 }
@@ -693,22 +713,28 @@ NormGrads qk_norm_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor
         "cott_qk_norm_bwd");
   return {dq, dk, dqw, dkw};
 }
-struct QKNormFn : torch::autograd::Function<QKNormFn> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& qw_, const at::Tensor& kw_,
-                               const OptTensor& sin, const OptTensor& cos, double eps) {
-    const at::Tensor q = rows16(q_), k = rows16(k_), qw = qw_.contiguous(), kw = kw_.contiguous();
+struct NormCall {
+  at::Tensor q, k, qw, kw, q_out, k_out;
+  Tables tab;
+  NormCall(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& qw_, const at::Tensor& kw_, const OptTensor& sin, const OptTensor& cos, double eps)
+      : q(rows16(q_)), k(rows16(k_)), qw(qw_.contiguous()), kw(kw_.contiguous()), tab(sin, cos, q) {
     const c10::cuda::CUDAGuard guard(q.device());
-    const Tables tab(sin, cos, q);
-    at::Tensor q_out = at::empty_like(q), k_out = at::empty_like(k);
+    q_out = at::empty_like(q), k_out = at::empty_like(k);
     cott_norm_layout lay = {};
     lay.q = strides3(q), lay.k = strides3(k), lay.q_out = strides3(q_out), lay.k_out = strides3(k_out);
     check(cott_qk_norm_fwd(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), tab.get(), q_out.data_ptr(), k_out.data_ptr(), &lay, (int)q.size(0),
                            (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)q.size(3), (float)eps, dtype_code(q.scalar_type()),
                            dtype_code(qw.scalar_type()), stream_of(q)),
           "cott_qk_norm_fwd");
-    ctx->save_for_backward({q, k, qw, kw, tab.sin, tab.cos});
+  }
+};
+struct QKNormFn : torch::autograd::Function<QKNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& qw_, const at::Tensor& kw_,
+                               const OptTensor& sin, const OptTensor& cos, double eps) {
+    const NormCall c(q_, k_, qw_, kw_, sin, cos, eps);
+    ctx->save_for_backward({c.q, c.k, c.qw, c.kw, c.tab.sin, c.tab.cos});
     ctx->saved_data["eps"] = eps;
-    return {q_out, k_out};
+    return {c.q_out, c.k_out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
@@ -741,6 +767,10 @@ variable_list qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at:
     TORCH_CHECK(w.sizes() == at::IntArrayRef({D}) && (w.scalar_type() == at::kFloat || w.scalar_type() == t) && w.scalar_type() == qw.scalar_type(),
                 "the weights must be [D] = [", D, "], both in float32 or both of the tensors' type, got ", w.sizes(), " in ", w.scalar_type());
   TORCH_CHECK(k.device() == q.device() && qw.device() == q.device() && kw.device() == q.device(), "q, k and the weights must be on one device");
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || qw.requires_grad() || kw.requires_grad())) {
+    const NormCall c(q, k, qw, kw, sin, cos, eps);
+    return {c.q_out, c.k_out};
+  }
   return QKNormFn::apply(q, k, qw, kw, sin, cos, eps);
 }
 
