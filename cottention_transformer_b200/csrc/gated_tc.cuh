@@ -509,25 +509,28 @@ __device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_l
   ptx::tmem_ld_x32(taddr_lane + 32 * blk, r);
   ptx::tmem_ld_wait();
   if (blk == wq) {
+    const uint32_t keep_bits = LOWER ? (2u << lane) - 1u : 0xffffffffu << lane;
+    const float sign = LOWER ? 1.f : -1.f;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 Gs = *reinterpret_cast<const float4*>(&sG[32 * blk + j]);
-      const float gs[4] = {Gs.x, Gs.y, Gs.z, Gs.w};
-      float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = LOWER ? j + e <= lane : j + e >= lane;
-        x[e] = in ? __uint_as_float(r[j + e]) * ex2(LOWER ? Gr - gs[e] : gs[e] - Gr) : 0.f;
+      for (int e = 0; e < 4; e += 2) {
+        float2 x = fma2(make_float2(-sign, -sign), e ? make_float2(Gs.z, Gs.w) : make_float2(Gs.x, Gs.y), make_float2(sign * Gr, sign * Gr));
+        x = mul2(make_float2(ex2(x.x), ex2(x.y)), pair(r + j + e));
+        x.x = keep_bits & (1u << (j + e)) ? x.x : 0.f;
+        x.y = keep_bits & (2u << (j + e)) ? x.y : 0.f;
+        pk[(j + e) / 2] = Pack2<T>::pack(x.x, x.y);
       }
-      pk[j / 2] = Pack2<T>::pack(x[0], x[1]);
-      pk[j / 2 + 1] = Pack2<T>::pack(x[2], x[3]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 cf = *reinterpret_cast<const float4*>(&col[32 * blk + j]);
-      pk[j / 2] = Pack2<T>::pack(__uint_as_float(r[j]) * (rowf * cf.x), __uint_as_float(r[j + 1]) * (rowf * cf.y));
-      pk[j / 2 + 1] = Pack2<T>::pack(__uint_as_float(r[j + 2]) * (rowf * cf.z), __uint_as_float(r[j + 3]) * (rowf * cf.w));
+      const float2 x = mul2(pair(r + j), mul2(make_float2(cf.x, cf.y), make_float2(rowf, rowf)));
+      const float2 y = mul2(pair(r + j + 2), mul2(make_float2(cf.z, cf.w), make_float2(rowf, rowf)));
+      pk[j / 2] = Pack2<T>::pack(x.x, x.y);
+      pk[j / 2 + 1] = Pack2<T>::pack(y.x, y.y);
     }
   }
 }
@@ -536,15 +539,25 @@ __device__ __forceinline__ void acc_scaled(float (&acc)[32], uint32_t taddr_lane
   uint32_t r[32];
   ptx::tmem_ld_x32(taddr_lane, r);
   ptx::tmem_ld_wait();
+  if (f == 0.f) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) acc[j] = f == 0.f ? 0.f : f * __uint_as_float(r[j]);
+    for (int j = 0; j < 32; ++j) r[j] = 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const float2 x = mul2(pair(r + j), make_float2(f, f));
+    acc[j] = x.x, acc[j + 1] = x.y;
+  }
 }
 __device__ __forceinline__ void acc_add(float (&acc)[32], uint32_t taddr_lane) {
   uint32_t r[32];
   ptx::tmem_ld_x32(taddr_lane, r);
   ptx::tmem_ld_wait();
 #pragma unroll
-  for (int j = 0; j < 32; ++j) acc[j] += __uint_as_float(r[j]);
+  for (int j = 0; j < 32; j += 2) {
+    const float2 x = fma2(pair(r + j), make_float2(1.f, 1.f), make_float2(acc[j], acc[j + 1]));
+    acc[j] = x.x, acc[j + 1] = x.y;
+  }
 }
 // 32 columns of a row -> pieces j0 .. j0 + 3 of a tile's row
 template <typename T>
@@ -559,18 +572,15 @@ __device__ __forceinline__ void stage_row(unsigned char* tile, int row, int j0, 
 }
 template <typename T>
 __device__ __forceinline__ float row_dot32(unsigned char* tile, int row, int j0, const float (&acc)[32]) {
-  float d = 0.f;
+  float2 d = make_float2(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint4 p = *tile_piece(tile, row, j0 + j);
     const uint32_t u[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = Pack2<T>::unpack(u[e]);
-      d = fmaf(f.x, acc[8 * j + 2 * e], fmaf(f.y, acc[8 * j + 2 * e + 1], d));
-    }
+    for (int e = 0; e < 4; ++e) d = fma2(Pack2<T>::unpack(u[e]), make_float2(acc[8 * j + 2 * e], acc[8 * j + 2 * e + 1]), d);
   }
-  return d;
+  return d.x + d.y;
 }
 
 constexpr int kFwdThreads = 256;

@@ -75,15 +75,34 @@ __device__ __forceinline__ float row_sum(float x) {
   for (int off = LPR / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
   return x;
 }
+// Two products, two multiply-adds in one instruction (the pass is as much bound by its instructions as by memory).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // the lane's E weights
 template <typename T, int E>
-__device__ __forceinline__ void load_weights(float (&w)[E], const void* src, int f32, int c) {
+__device__ __forceinline__ void load_weights(float2 (&w)[E / 2], const void* src, int f32, int c) {
+  float x[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) w[e] = f32 ? static_cast<const float*>(src)[c + e] : to_acc(static_cast<const T*>(src)[c + e]);
+  for (int e = 0; e < E; ++e) x[e] = f32 ? static_cast<const float*>(src)[c + e] : to_acc(static_cast<const T*>(src)[c + e]);
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) w[e] = make_float2(x[2 * e], x[2 * e + 1]);
 }
 // rotates the lane's E/2 pairs; `sign` = -1: the transposed rotation
 template <int E>
-__device__ __forceinline__ void rotate(float (&x)[E], const float* sin_t, const float* cos_t, float sign) {
+__device__ __forceinline__ void rotate(float2 (&x)[E / 2], const float* sin_t, const float* cos_t, float sign) {
   float s[E / 2], c[E / 2];
   if constexpr (E == 8) {
     *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_t);
@@ -93,11 +112,7 @@ __device__ __forceinline__ void rotate(float (&x)[E], const float* sin_t, const 
     *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cos_t);
   }
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) {
-    float xo, yo;
-    rot_pair(x[2 * i], x[2 * i + 1], c[i], sign * s[i], xo, yo);
-    x[2 * i] = xo, x[2 * i + 1] = yo;
-  }
+  for (int i = 0; i < E / 2; ++i) x[i] = fma2(x[i], both(c[i]), mul2(make_float2(x[i].y, x[i].x), make_float2(-sign * s[i], sign * s[i])));
 }
 
 // grid = (CTAs, 2): y = q, k.  A CTA takes U groups of rows at a time, all of whose loads are in flight together: with one group
@@ -109,7 +124,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_fwd_kernel(const NormArg
   const int piece = threadIdx.x % LPR, c = piece * E;
   pdl_allow_next();
   pdl_wait_prior();
-  float w[E];
+  float2 w[E / 2];
   load_weights<T, E>(w, s.w, a.w_f32, c);
   for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
     RowAt row[U];
@@ -122,21 +137,21 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_fwd_kernel(const NormArg
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float x[E], sum = 0.f;
+      float2 x[E / 2], sum = both(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] = to_acc(p[u].e[e]);
-        sum = fmaf(x[e], x[e], sum);
+      for (int e = 0; e < E / 2; ++e) {
+        x[e] = make_float2(to_acc(p[u].e[2 * e]), to_acc(p[u].e[2 * e + 1]));
+        sum = fma2(x[e], x[e], sum);
       }
-      const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
+      const float rms = rsqrtf(row_sum<LPR>(sum.x + sum.y) * (1.f / D) + a.eps);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = x[e] * rms * w[e];
+      for (int e = 0; e < E / 2; ++e) x[e] = mul2(mul2(x[e], both(rms)), w[e]);
       if (c < a.rot) {
         const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
         rotate<E>(x, a.sin_t + t, a.cos_t + t, 1.f);
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) p[u].e[e] = from_acc<T>(x[e]);
+      for (int e = 0; e < E / 2; ++e) p[u].e[2 * e] = from_acc<T>(x[e].x), p[u].e[2 * e + 1] = from_acc<T>(x[e].y);
       if (r0 + u * RPC + threadIdx.x / LPR < s.rows) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row[u]) + c) = p[u].u;
     }
   }
@@ -150,10 +165,10 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArg
   __shared__ float part[RPC][D];
   pdl_allow_next();
   pdl_wait_prior();
-  float w[E], dw[E];
+  float2 w[E / 2], dw[E / 2];
   load_weights<T, E>(w, s.w, a.w_f32, c);
 #pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = 0.f;
+  for (int e = 0; e < E / 2; ++e) dw[e] = both(0.f);
   for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
     RowAt row[U];
     Piece<T> p[U], d[U];
@@ -167,34 +182,37 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArg
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = r0 + u * RPC + threadIdx.x / LPR < s.rows;
-      float x[E], f[E], sum = 0.f;
+      float2 x[E / 2], f[E / 2], sum = both(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] = to_acc(p[u].e[e]);
-        f[e] = to_acc(d[u].e[e]);
-        sum = fmaf(x[e], x[e], sum);
+      for (int e = 0; e < E / 2; ++e) {
+        x[e] = make_float2(to_acc(p[u].e[2 * e]), to_acc(p[u].e[2 * e + 1]));
+        f[e] = make_float2(to_acc(d[u].e[2 * e]), to_acc(d[u].e[2 * e + 1]));
+        sum = fma2(x[e], x[e], sum);
       }
       if (c < a.rot) {
         const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
         rotate<E>(f, a.sin_t + t, a.cos_t + t, -1.f);
       }
-      const float rms = rsqrtf(row_sum<LPR>(sum) * (1.f / D) + a.eps);
-      float dot = 0.f;
+      const float rms = rsqrtf(row_sum<LPR>(sum.x + sum.y) * (1.f / D) + a.eps);
+      float2 dot2 = both(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] *= rms;
-        if (in) dw[e] = fmaf(f[e], x[e], dw[e]);
-        f[e] *= w[e];
-        dot = fmaf(f[e], x[e], dot);
+      for (int e = 0; e < E / 2; ++e) {
+        x[e] = mul2(x[e], both(rms));
+        if (in) dw[e] = fma2(f[e], x[e], dw[e]);
+        f[e] = mul2(f[e], w[e]);
+        dot2 = fma2(f[e], x[e], dot2);
       }
-      dot = row_sum<LPR>(dot) * (1.f / D);
+      const float dot = row_sum<LPR>(dot2.x + dot2.y) * (1.f / D);
 #pragma unroll
-      for (int e = 0; e < E; ++e) p[u].e[e] = from_acc<T>(rms * (f[e] - x[e] * dot));
+      for (int e = 0; e < E / 2; ++e) {
+        const float2 g = mul2(fma2(x[e], both(-dot), f[e]), both(rms));
+        p[u].e[2 * e] = from_acc<T>(g.x), p[u].e[2 * e + 1] = from_acc<T>(g.y);
+      }
       if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row[u]) + c) = p[u].u;
     }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) part[threadIdx.x / LPR][c + e] = dw[e];
+  for (int e = 0; e < E / 2; ++e) part[threadIdx.x / LPR][c + 2 * e] = dw[e].x, part[threadIdx.x / LPR][c + 2 * e + 1] = dw[e].y;
   __syncthreads();
   for (int e = threadIdx.x; e < D; e += kNormThreads) {
     float sum = 0.f;
