@@ -745,6 +745,7 @@ struct GatedMaps {
   CUtensorMap q, k, v, o, dq, dk, dv;
 };
 template <int D> constexpr int bwd_threads() { return 4 * D; }
+constexpr int kBwdAhead = 148;  // units: a CTA on each SM
 template <int D> constexpr size_t bwd_tc_smem() { return 1024 + 4 * (D / 64) * kTileBytes + 2 * (D / 64) * (D / 64) * kStateTile; }
 
 // Backward of one chunk: dq, dk, dv and dg from q, k, v, dO and the two states, each read once; grid = B*H * chunks.
@@ -824,6 +825,18 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
       }
       if (with_S) bulk_load(sS, a.S + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
       if (with_R) bulk_load(sR, a.R + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
+      const long next = unit + kBwdAhead;  // the tiles of the CTA that takes this one's place, into L2
+      if (next < a.units) {
+        const long nbh = next / a.nchunks;
+        const int ny = static_cast<int>(next % a.nchunks) * kGtChunk, nh = static_cast<int>(nbh % a.H), nb = static_cast<int>(nbh / a.H);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          tma_prefetch_tile_x(&m.o, 64 * i, ny, nh, nb);
+          tma_prefetch_tile_x(&m.v, 64 * i, ny, nh, nb);
+          tma_prefetch_tile_x(&m.k, 64 * i, ny, nh, nb);
+          tma_prefetch_tile_x(&m.q, 64 * i, ny, nh, nb);
+        }
+      }
     }
     __syncwarp();
   } else if (warp == 4) {

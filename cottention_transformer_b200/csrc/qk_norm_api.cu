@@ -14,6 +14,8 @@ using namespace cott;
 namespace {
 
 constexpr int kNormThreads = 256;
+constexpr int kSms = 148, kFwdResident = 4, kBwdResident = 3;  // CTAs per SM, by their registers
+constexpr int kFwdStages = 3, kBwdStages = 2;
 
 template <typename T> struct Piece {
   static constexpr int kElems = 16 / sizeof(T);
@@ -68,6 +70,13 @@ __device__ __forceinline__ RowAt row_at(unsigned r, const Divider& heads, const 
   return RowAt{b, p - b * positions.d, r - p * heads.d};
 }
 __device__ __forceinline__ long long at(const cott_strides& s, const RowAt& r) { return r.b * s.b + r.h * s.h + r.n * s.n; }
+// A piece of 16 bytes of this thread's own, from global to its place in shared memory without a register in between.
+__device__ __forceinline__ void fetch16(void* smem, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x) {
@@ -100,125 +109,137 @@ __device__ __forceinline__ void load_weights(float2 (&w)[E / 2], const void* src
 #pragma unroll
   for (int e = 0; e < E / 2; ++e) w[e] = make_float2(x[2 * e], x[2 * e + 1]);
 }
-// rotates the lane's E/2 pairs; `sign` = -1: the transposed rotation
-template <int E>
-__device__ __forceinline__ void rotate(float2 (&x)[E / 2], const float* sin_t, const float* cos_t, float sign) {
+// a position's sines and cosines of the lane's E/2 pairs; apply() rotates, `sign` = -1: by the transposed rotation
+template <int E> struct Turn {
   float s[E / 2], c[E / 2];
-  if constexpr (E == 8) {
-    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_t);
-    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cos_t);
-  } else {
-    *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(sin_t);
-    *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cos_t);
+  __device__ __forceinline__ void load(const float* sin_t, const float* cos_t) {
+    if constexpr (E == 8) {
+      *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_t);
+      *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cos_t);
+    } else {
+      *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(sin_t);
+      *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cos_t);
+    }
   }
+  __device__ __forceinline__ void apply(float2 (&x)[E / 2], float sign) const {
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) x[i] = fma2(x[i], both(c[i]), mul2(make_float2(x[i].y, x[i].x), make_float2(-sign * s[i], sign * s[i])));
-}
+    for (int i = 0; i < E / 2; ++i) x[i] = fma2(x[i], both(c[i]), mul2(make_float2(x[i].y, x[i].x), make_float2(-sign * s[i], sign * s[i])));
+  }
+};
 
-// grid = (CTAs, 2): y = q, k.  A CTA takes U groups of rows at a time, all of whose loads are in flight together: with one group
-// the pass reached 3.6 TB/s.
-template <typename T, int D, int U>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_fwd_kernel(const NormArgs a) {
-  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;  // elements and lanes of a piece, rows per group
-  const NormSide& s = a.side[blockIdx.y];
-  const int piece = threadIdx.x % LPR, c = piece * E;
+// Both passes.  A thread always has the same piece of a row, and takes every so many-th row: of q and of k both (SIDES = 2: as many
+// heads in one as in the other), which share the position's table entries, or of one of them (SIDES = 1: blockIdx.x even q, odd k).
+// The pieces of the next STAGES rows are on their way while one is worked on: each thread fetches its own into its own places in
+// shared memory, so nobody waits for anybody else.
+// B8 H16 N4096, q and k of a packed projection, us forward / backward: one row at a time 74 / 123, four and two rows loaded together
+// 60 / 90, fetched ahead 63 / 89 (46 without the rotation: the tables were twice the data), q and k together 46 / 73.
+template <typename T, int D, bool BWD, int STAGES, int SIDES>
+__global__ void __launch_bounds__(kNormThreads, STAGES == 1 ? 1 : BWD ? kBwdResident : kFwdResident) qk_norm_kernel(const NormArgs a) {
+  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;  // elements and lanes of a piece, rows per round
+  const int first_side = SIDES == 2 ? 0 : blockIdx.x & 1, cta = SIDES == 2 ? blockIdx.x : blockIdx.x >> 1, ctas = SIDES == 2 ? gridDim.x : gridDim.x >> 1;
+  const int c = threadIdx.x % LPR * E;
+  const unsigned group = RPC * ctas, rows = a.side[first_side].rows;
+  extern __shared__ __align__(16) unsigned char norm_smem[];  // pieces [STAGES][SIDES][x, dy][threads]; at the end [RPC][D] sums
+  uint4* buf = reinterpret_cast<uint4*>(norm_smem) + threadIdx.x;
+  auto place = [&](int stage, int i, int dy) { return buf + ((stage * SIDES + i) * (BWD ? 2 : 1) + dy) * kNormThreads; };
   pdl_allow_next();
   pdl_wait_prior();
-  float2 w[E / 2];
-  load_weights<T, E>(w, s.w, a.w_f32, c);
-  for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
-    RowAt row[U];
-    Piece<T> p[U];
+  float2 w[SIDES][E / 2], dw[SIDES][E / 2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned r = r0 + u * RPC + threadIdx.x / LPR;
-      row[u] = row_at(r < s.rows ? r : s.rows - 1, s.heads, a.positions);
-      p[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row[u]) + c);
+  for (int i = 0; i < SIDES; ++i) {
+    load_weights<T, E>(w[i], a.side[first_side + i].w, a.w_f32, c);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) dw[i][e] = both(0.f);
+  }
+  auto fetch = [&](unsigned r, int stage) {
+    if (r < rows) {
+      const RowAt row = row_at(r, a.side[first_side].heads, a.positions);
+#pragma unroll
+      for (int i = 0; i < SIDES; ++i) {
+        const NormSide& s = a.side[first_side + i];
+        fetch16(place(stage, i, 0), static_cast<const T*>(s.x) + at(s.sx, row) + c);
+        if constexpr (BWD) fetch16(place(stage, i, 1), static_cast<const T*>(s.dy) + at(s.sdy, row) + c);
+      }
     }
+    fetch_commit();
+  };
+  const unsigned first = cta * RPC + threadIdx.x / LPR;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+  for (int i = 0; i < STAGES; ++i) fetch(first + i * group, i);
+  int stage = 0;
+  // (as many rounds for every lane of a warp: the rows' sums are exchanged by all)
+  for (unsigned r = first; __any_sync(0xffffffffu, r < rows); r += group) {
+    fetch_wait<STAGES - 1>();
+    Piece<T> p[SIDES], d[SIDES];
+#pragma unroll
+    for (int i = 0; i < SIDES; ++i) {
+      p[i].u = *place(stage, i, 0);
+      if constexpr (BWD) d[i].u = *place(stage, i, 1);
+    }
+    const bool in = r < rows, turned = c < a.rot;  // (the same for all lanes of a row)
+    const RowAt row = row_at(in ? r : rows - 1, a.side[first_side].heads, a.positions);
+    Turn<E> turn;
+    if (turned) {
+      const long long t = row.b * a.table_batch_stride + static_cast<long long>(row.n) * (a.rot / 2) + c / 2;
+      turn.load(a.sin_t + t, a.cos_t + t);
+    }
+    fetch(r + STAGES * group, stage);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+    for (int i = 0; i < SIDES; ++i) {
+      const NormSide& s = a.side[first_side + i];
       float2 x[E / 2], sum = both(0.f);
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
-        x[e] = make_float2(to_acc(p[u].e[2 * e]), to_acc(p[u].e[2 * e + 1]));
+        x[e] = make_float2(to_acc(p[i].e[2 * e]), to_acc(p[i].e[2 * e + 1]));
         sum = fma2(x[e], x[e], sum);
       }
       const float rms = rsqrtf(row_sum<LPR>(sum.x + sum.y) * (1.f / D) + a.eps);
+      if constexpr (!BWD) {
 #pragma unroll
-      for (int e = 0; e < E / 2; ++e) x[e] = mul2(mul2(x[e], both(rms)), w[e]);
-      if (c < a.rot) {
-        const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
-        rotate<E>(x, a.sin_t + t, a.cos_t + t, 1.f);
+        for (int e = 0; e < E / 2; ++e) x[e] = mul2(mul2(x[e], both(rms)), w[i][e]);
+        if (turned) turn.apply(x, 1.f);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) p[i].e[2 * e] = from_acc<T>(x[e].x), p[i].e[2 * e + 1] = from_acc<T>(x[e].y);
+        if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row) + c) = p[i].u;
+      } else {
+        float2 f[E / 2], dot2 = both(0.f);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) f[e] = make_float2(to_acc(d[i].e[2 * e]), to_acc(d[i].e[2 * e + 1]));
+        if (turned) turn.apply(f, -1.f);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          x[e] = mul2(x[e], both(rms));
+          if (in) dw[i][e] = fma2(f[e], x[e], dw[i][e]);
+          f[e] = mul2(f[e], w[i][e]);
+          dot2 = fma2(f[e], x[e], dot2);
+        }
+        const float dot = row_sum<LPR>(dot2.x + dot2.y) * (1.f / D);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          const float2 g = mul2(fma2(x[e], both(-dot), f[e]), both(rms));
+          p[i].e[2 * e] = from_acc<T>(g.x), p[i].e[2 * e + 1] = from_acc<T>(g.y);
+        }
+        if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row) + c) = p[i].u;
       }
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) p[u].e[2 * e] = from_acc<T>(x[e].x), p[u].e[2 * e + 1] = from_acc<T>(x[e].y);
-      if (r0 + u * RPC + threadIdx.x / LPR < s.rows) *reinterpret_cast<uint4*>(static_cast<T*>(s.y) + at(s.sy, row[u]) + c) = p[u].u;
     }
   }
-}
-
-template <typename T, int D, int U>
-__global__ void __launch_bounds__(kNormThreads) qk_norm_bwd_kernel(const NormArgs a) {
-  constexpr int E = Piece<T>::kElems, LPR = D / E, RPC = kNormThreads / LPR;
-  const NormSide& s = a.side[blockIdx.y];
-  const int piece = threadIdx.x % LPR, c = piece * E;
-  __shared__ float part[RPC][D];
-  pdl_allow_next();
-  pdl_wait_prior();
-  float2 w[E / 2], dw[E / 2];
-  load_weights<T, E>(w, s.w, a.w_f32, c);
+  fetch_wait<0>();
+  if constexpr (BWD) {
+    float(*part)[D] = reinterpret_cast<float(*)[D]>(norm_smem);
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) dw[e] = both(0.f);
-  for (unsigned r0 = blockIdx.x * (RPC * U); r0 < s.rows; r0 += gridDim.x * (RPC * U)) {
-    RowAt row[U];
-    Piece<T> p[U], d[U];
+    for (int i = 0; i < SIDES; ++i) {
+      __syncthreads();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned r = r0 + u * RPC + threadIdx.x / LPR;
-      row[u] = row_at(r < s.rows ? r : s.rows - 1, s.heads, a.positions);
-      p[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.x) + at(s.sx, row[u]) + c);
-      d[u].u = *reinterpret_cast<const uint4*>(static_cast<const T*>(s.dy) + at(s.sdy, row[u]) + c);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = r0 + u * RPC + threadIdx.x / LPR < s.rows;
-      float2 x[E / 2], f[E / 2], sum = both(0.f);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        x[e] = make_float2(to_acc(p[u].e[2 * e]), to_acc(p[u].e[2 * e + 1]));
-        f[e] = make_float2(to_acc(d[u].e[2 * e]), to_acc(d[u].e[2 * e + 1]));
-        sum = fma2(x[e], x[e], sum);
-      }
-      if (c < a.rot) {
-        const long long t = row[u].b * a.table_batch_stride + static_cast<long long>(row[u].n) * (a.rot / 2) + c / 2;
-        rotate<E>(f, a.sin_t + t, a.cos_t + t, -1.f);
-      }
-      const float rms = rsqrtf(row_sum<LPR>(sum.x + sum.y) * (1.f / D) + a.eps);
-      float2 dot2 = both(0.f);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        x[e] = mul2(x[e], both(rms));
-        if (in) dw[e] = fma2(f[e], x[e], dw[e]);
-        f[e] = mul2(f[e], w[e]);
-        dot2 = fma2(f[e], x[e], dot2);
-      }
-      const float dot = row_sum<LPR>(dot2.x + dot2.y) * (1.f / D);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        const float2 g = mul2(fma2(x[e], both(-dot), f[e]), both(rms));
-        p[u].e[2 * e] = from_acc<T>(g.x), p[u].e[2 * e + 1] = from_acc<T>(g.y);
-      }
-      if (in) *reinterpret_cast<uint4*>(static_cast<T*>(s.dx) + at(s.sdx, row[u]) + c) = p[u].u;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E / 2; ++e) part[threadIdx.x / LPR][c + 2 * e] = dw[e].x, part[threadIdx.x / LPR][c + 2 * e + 1] = dw[e].y;
-  __syncthreads();
-  for (int e = threadIdx.x; e < D; e += kNormThreads) {
-    float sum = 0.f;
+      for (int e = 0; e < E / 2; ++e) part[threadIdx.x / LPR][c + 2 * e] = dw[i][e].x, part[threadIdx.x / LPR][c + 2 * e + 1] = dw[i][e].y;
+      __syncthreads();
+      for (int e = threadIdx.x; e < D; e += kNormThreads) {
+        float sum = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < RPC; ++i) sum += part[i][e];
-    a.partial[(static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x) * D + e] = sum;
+        for (int k = 0; k < RPC; ++k) sum += part[k][e];
+        a.partial[(static_cast<long>(first_side + i) * ctas + cta) * D + e] = sum;
+      }
+    }
   }
 }
 
@@ -272,28 +293,35 @@ int check_norm_rows(const char* name, const void* p, const cott_strides& s, int 
   return COTT_OK;
 }
 
-int norm_ctas(unsigned rows, int rows_per_cta, int resident) {
-  int sm = 148, dev = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, dev);
-  const long want = ((long)rows + rows_per_cta - 1) / rows_per_cta, most = (long)sm * resident;
+// CTAs of one side (of both, where a CTA takes both): one wave, at most one per round of rows
+int norm_ctas(unsigned rows, int rows_per_round, int resident) {
+  const long want = ((long)rows + rows_per_round - 1) / rows_per_round, most = kSms * resident;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
-constexpr int kBwdResident = 4, kFwdGroups = 4, kBwdGroups = 2;
 
+template <typename T, int D, bool BWD, int STAGES, int SIDES>
+int launch_norm_as(const NormArgs& a, int ctas, cudaStream_t stream) {
+  constexpr int RPC = kNormThreads / (D / Piece<T>::kElems);
+  const int pieces = STAGES * SIDES * (BWD ? 2 : 1) * kNormThreads * 16, sums = BWD ? RPC * D * 4 : 0;
+  auto kern = qk_norm_kernel<T, D, BWD, STAGES, SIDES>;
+  const size_t smem = pieces > sums ? pieces : sums;
+  if (smem > 48 * 1024) COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  COTT_CUDA_TRY(launch_pdl(kern, dim3(SIDES == 2 ? ctas : 2 * ctas), kNormThreads, smem, stream, a));
+  return COTT_OK;
+}
 template <typename T, int D>
 int launch_norm(const NormArgs& a, bool bwd, void* dqw, void* dkw, cudaStream_t stream) {
   constexpr int RPC = kNormThreads / (D / Piece<T>::kElems);
+  const bool same = a.side[0].rows == a.side[1].rows;
   const unsigned rows = a.side[0].rows > a.side[1].rows ? a.side[0].rows : a.side[1].rows;
+  const int ctas = norm_ctas(rows, RPC, same ? (bwd ? kBwdResident : kFwdResident) : (bwd ? kBwdResident : kFwdResident) / 2);
   if (!bwd) {
-    // (few rows, as of new tokens: one group per CTA, so that they are spread over the SMs)
-    if (rows <= 148u * RPC)
-      COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D, 1>, dim3(norm_ctas(rows, RPC, 64), 2), kNormThreads, 0, stream, a));
-    else
-      COTT_CUDA_TRY(launch_pdl(qk_norm_fwd_kernel<T, D, kFwdGroups>, dim3(norm_ctas(rows, RPC * kFwdGroups, 64), 2), kNormThreads, 0, stream, a));
-    return COTT_OK;
+    // few rows, as of new tokens: nothing to fetch ahead, and q and k on CTAs of their own
+    if ((long)kSms * RPC >= rows) return launch_norm_as<T, D, false, 1, 1>(a, norm_ctas(rows, RPC, 1), stream);
+    return same ? launch_norm_as<T, D, false, kFwdStages, 2>(a, ctas, stream) : launch_norm_as<T, D, false, kFwdStages, 1>(a, ctas, stream);
   }
-  const int ctas = norm_ctas(rows, RPC * kBwdGroups, kBwdResident);
-  COTT_CUDA_TRY(launch_pdl(qk_norm_bwd_kernel<T, D, kBwdGroups>, dim3(ctas, 2), kNormThreads, 0, stream, a));
+  const int st = same ? launch_norm_as<T, D, true, kBwdStages, 2>(a, ctas, stream) : launch_norm_as<T, D, true, kBwdStages, 1>(a, ctas, stream);
+  if (st) return st;
   COTT_CUDA_TRY(launch_pdl(qk_norm_dw_kernel<T>, dim3(D / 32, 2), 1024, 0, stream, static_cast<const float*>(a.partial), dqw, dkw, ctas, D, a.w_f32));
   return COTT_OK;
 }
