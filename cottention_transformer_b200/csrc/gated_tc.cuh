@@ -37,7 +37,7 @@ struct GatedTcArgs {
   float* last;              // [B*H][value][key]: the state after its last one, or null
   unsigned char* states;    // [B*H][nchunks][D/64] swizzled [D x 64] panels (key x value); c: before chunk c (REV: after it)
   float* seg_state;         // [B*H][D/64][segments][D][64]: sums of the segments, then the states before them
-  float* seg_log;           // [B*H][segments]
+  float *seg_log, *chunk_log;  // [B*H][segments], [B*H][nchunks]: log2 of the decay over a segment, from its start to a chunk
   int H, N, nchunks, chunks_per_seg, nseg, gate_f32;
 };
 
@@ -177,13 +177,15 @@ template <int D, int SPLIT> constexpr int walk_stages() { return 192 * 1024 / wa
 template <int D, int SPLIT> constexpr size_t walk_smem() { return 1024 + walk_stages<D, SPLIT>() * walk_stage_bytes<D, SPLIT>() + 2 * (D / 64) * kStateTile; }
 
 // grid = (B*H, segments, D/64): one CTA owns 64 value columns of a segment's state.  Y = K, Z = V, or REV: Y = Q, Z = dO and the
-// chunks and segments are numbered from the end of the sequence.  EMIT: starts from the segment's state and leaves the state
-// before every chunk; else it sums the segment up, from zero.
+// chunks and segments are numbered from the end of the sequence.  A walk in segments starts each of them from nothing and leaves
+// their sums, from which gated_seg_kernel makes the states before them, and gated_patch_kernel adds those, decayed, to the states
+// inside.  (Walking a second time from the right states instead reads both tensors again: 62 us of 640 for a direction of B1 H16
+// N65536.)
 //   warps 0-3: state (fp32, in registers: a row of it per thread)    warp 8: TMA    warp 9: MMA
 //   warps 4-7, 10-13: weighted operand of the even / odd chunks
 // SPLIT: into how many 16-bit numbers the weighted operand is split.  Two where the states are wanted as 16-bit operands, three
 // where the last one is a result: it is then what fp32 products give.
-template <typename T, int D, bool REV, bool EMIT, int SPLIT>
+template <typename T, int D, bool REV, int SPLIT>
 __global__ void __launch_bounds__(kWalkThreads, 1)
 gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constant__ CUtensorMap mapZ, const GatedTcArgs a) {
   using namespace ptx;
@@ -209,7 +211,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
   auto chunk_at = [&](int c) { return REV ? a.nchunks - 1 - (chunk0 + c) : chunk0 + c; };
   const bool last_seg = seg + 1 == a.nseg;
   // the last chunk's own part is wanted only where somebody asks for the state after it
-  const int updates = !EMIT || (last_seg && a.last) ? nchunks : nchunks - 1;
+  const int updates = !last_seg || a.last ? nchunks : nchunks - 1;
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&bar_full[s], 1);
@@ -338,13 +340,7 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     float* seg_row = a.nseg > 1 ? a.seg_state + (((bh * NT + J) * a.nseg + seg) * D + i) * 64 : nullptr;
 #pragma unroll
     for (int j = 0; j < 64; ++j) S[j] = 0.f;
-    if (EMIT && a.nseg > 1) {
-#pragma unroll
-      for (int j = 0; j < 64; j += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(seg_row + j);
-        S[j] = f.x, S[j + 1] = f.y, S[j + 2] = f.z, S[j + 3] = f.w;
-      }
-    } else if (EMIT && a.edge) {
+    if (a.nseg == 1 && a.edge) {
 #pragma unroll
       for (int j = 0; j < 64; ++j) S[j] = a.edge[edge + static_cast<long>(j) * D];
     }
@@ -373,7 +369,8 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
     };
     bool ok = true;
     for (int c = 0; c < nchunks; ++c) {
-      if (EMIT) emit(chunk_at(c), c);
+      emit(chunk_at(c), c);
+      if (a.nseg > 1 && J == 0 && tid == 0) a.chunk_log[bh * a.nchunks + chunk_at(c)] = log_sum;
       if (c >= updates) break;
       if (!(ok = wait_bar2_warp(&bar_u_full[c & 1], (c >> 1) & 1, &bar_sum[c % NSUM], (c / NSUM) & 1, abort_flag, kWaitWalkState, c))) break;
       const float total = sSum[c % NSUM], A = ex2(total);
@@ -400,17 +397,19 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
       tc_fence_before_sync();
       warp_arrive(&bar_u_free[c & 1], lane);
     }
-    if (!EMIT) {
-      if (ok && mine) {
+    if (ok && updates == nchunks) {
+      if (a.nseg > 1) {
+        if (mine) {
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(seg_row + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+          for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(seg_row + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+        }
+        if (J == 0 && tid == 0) a.seg_log[bh * a.nseg + seg] = log_sum;
+      } else if (mine) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) a.last[edge + static_cast<long>(j) * D] = S[j];
       }
-      if (J == 0 && tid == 0) a.seg_log[bh * a.nseg + seg] = log_sum;
-    } else if (last_seg && ok && a.last && mine) {
-#pragma unroll
-      for (int j = 0; j < 64; ++j) a.last[edge + static_cast<long>(j) * D] = S[j];
     }
-    if (EMIT && lane == 0) tma_store_wait<0>();
+    if (lane == 0) tma_store_wait<0>();
   }
 
   __syncwarp();
@@ -423,7 +422,8 @@ gated_walk_kernel(const __grid_constant__ CUtensorMap mapY, const __grid_constan
   if (warp == 9) tmem_dealloc(tU, kCols);
 }
 
-// The states before the segments, in place of their sums: run <- e^(log) run + sum.  grid = (B*H * D/64, D * 64 / 256).
+// The states before the segments, in place of their sums, and the state after all of them: run <- e^(log) run + sum.
+// grid = (B*H * D/64, D * 64 / 256).  (The last sum is there only where the last state is wanted.)
 template <int D>
 __global__ void __launch_bounds__(256) gated_seg_kernel(const GatedTcArgs a) {
   constexpr int NT = D / 64;
@@ -444,8 +444,39 @@ __global__ void __launch_bounds__(256) gated_seg_kernel(const GatedTcArgs a) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       if (s + u < a.nseg) p[static_cast<long>(s + u) * (D * 64)] = run;
-      run = d[u] == 0.f ? x[u] : fmaf(d[u], run, x[u]);
+      if (s + u < a.nseg) run = d[u] == 0.f ? x[u] : fmaf(d[u], run, x[u]);
     }
+  }
+  if (a.last) a.last[bh * static_cast<long>(D * D) + (64 * J + j) * D + i] = run;
+}
+
+// The states inside a segment += the decayed state before it.  A CTA per chunk and panel; most of those of a head that forgets within
+// a segment have nothing to do.  grid = B*H * nchunks * D/64, block = 128.
+template <typename T, int D, bool REV>
+__global__ void __launch_bounds__(128) gated_patch_kernel(const GatedTcArgs a) {
+  constexpr int NT = D / 64;
+  const long unit = blockIdx.x / NT, bh = unit / a.nchunks;
+  const int J = static_cast<int>(blockIdx.x % NT), chunk = static_cast<int>(unit % a.nchunks), seg = (REV ? a.nchunks - 1 - chunk : chunk) / a.chunks_per_seg;
+  pdl_allow_next();
+  pdl_wait_prior();
+  if (seg == 0 && !a.edge) return;
+  const float f = ex2(a.chunk_log[unit]);
+  if (f == 0.f) return;
+  unsigned char* panel = a.states + (unit * NT + J) * static_cast<long>(NT * kStateTile);
+  const float* start = a.seg_state + ((bh * NT + J) * a.nseg + seg) * static_cast<long>(D * 64);
+#pragma unroll
+  for (int e = threadIdx.x; e < D * 8; e += 128) {  // piece e % 8 of row e / 8
+    uint4* p = tile_piece(panel, e >> 3, e & 7);
+    const float4 x = *reinterpret_cast<const float4*>(start + 8 * e), y = *reinterpret_cast<const float4*>(start + 8 * e + 4);
+    uint4 u = *p;
+    const float s[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 l = Pack2<T>::unpack(w[i]);
+      w[i] = Pack2<T>::pack(fmaf(f, s[2 * i], l.x), fmaf(f, s[2 * i + 1], l.y));
+    }
+    *p = u;
   }
 }
 

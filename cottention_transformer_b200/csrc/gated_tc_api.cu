@@ -9,20 +9,20 @@ constexpr int kSms = 148;  // (sizes of buffers follow from it: a constant, so t
 
 int tc_chunks(int N) { return (N + kGtChunk - 1) / kGtChunk; }
 
-// Into how many segments the walk of a sequence is cut: as many as there are SMs to spare, where the extra pass that sums the
-// segments up costs less than the cut saves.  In units of a chunk's time (about 0.4 us): n against twice n / segments, a launch and the
-// prefix (14).
+// Into how many segments the walk of a sequence is cut: as many as there are SMs to spare, where that saves more than the two short
+// kernels behind it cost (a chunk of a walk takes about 1 us, they take about 10).
 int walk_segments(long walks, int n) {
   const int room = (int)(kSms / walks);
-  if (room < 3) return 1;
+  if (room < 2) return 1;
   const int per = (n + room - 1) / room;
-  if (n <= 2 * per + 14) return 1;
-  return (n + per - 1) / per;
+  return n - per < 10 ? 1 : (n + per - 1) / per;
 }
 size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 size_t seg_bytes(long bh, int N, int D) {
   const int nseg = walk_segments(bh * (D / 64), tc_chunks(N));
-  return nseg > 1 ? round256((size_t)bh * nseg * D * D * sizeof(float)) + round256((size_t)bh * nseg * sizeof(float)) : 0;
+  return nseg > 1 ? round256((size_t)bh * nseg * D * D * sizeof(float)) + round256((size_t)bh * nseg * sizeof(float)) +
+                        round256((size_t)bh * tc_chunks(N) * sizeof(float))
+                  : 0;
 }
 size_t tile_bytes(int D) { return (size_t)(D / 64) * (D / 64) * kStateTile; }
 
@@ -52,16 +52,19 @@ int launch_walk_split(GatedTcArgs a, const CUtensorMap& y, const CUtensorMap& z,
   a.chunks_per_seg = (a.nchunks + a.nseg - 1) / a.nseg;
   const dim3 grid((unsigned)bh, a.nseg, NT);
   if (a.nseg > 1) {
-    a.seg_state = static_cast<float*>(seg);
-    a.seg_log = reinterpret_cast<float*>(static_cast<unsigned char*>(seg) + round256((size_t)bh * a.nseg * D * D * sizeof(float)));
-    auto sum = gated_walk_kernel<T, D, REV, false, SPLIT>;
-    COTT_CUDA_TRY(cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    COTT_CUDA_TRY(launch_pdl(sum, grid, kWalkThreads, smem, stream, y, z, a));
-    COTT_CUDA_TRY(launch_pdl(gated_seg_kernel<D>, dim3((unsigned)(bh * NT), D * 64 / 256), 256, 0, stream, a));
+    unsigned char* p = static_cast<unsigned char*>(seg);
+    a.seg_state = reinterpret_cast<float*>(p);
+    p += round256((size_t)bh * a.nseg * D * D * sizeof(float));
+    a.seg_log = reinterpret_cast<float*>(p);
+    a.chunk_log = reinterpret_cast<float*>(p + round256((size_t)bh * a.nseg * sizeof(float)));
   }
-  auto walk = gated_walk_kernel<T, D, REV, true, SPLIT>;
+  auto walk = gated_walk_kernel<T, D, REV, SPLIT>;
   COTT_CUDA_TRY(cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   COTT_CUDA_TRY(launch_pdl(walk, grid, kWalkThreads, smem, stream, y, z, a));
+  if (a.nseg > 1) {
+    COTT_CUDA_TRY(launch_pdl(gated_seg_kernel<D>, dim3((unsigned)(bh * NT), D * 64 / 256), 256, 0, stream, a));
+    COTT_CUDA_TRY(launch_pdl(gated_patch_kernel<T, D, REV>, dim3((unsigned)(bh * a.nchunks * NT)), 128, 0, stream, a));
+  }
   return COTT_OK;
 }
 template <typename T, int D, bool REV>

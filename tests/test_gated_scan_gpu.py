@@ -66,7 +66,8 @@ def _compare(got, want, dtype):
 
 SHAPES = [(1, 1, 1, 64), (1, 2, 2, 128), (2, 3, 63, 32), (1, 2, 64, 64), (2, 2, 65, 64), (1, 2, 127, 128), (1, 2, 128, 64), (1, 3, 129, 128),
           (2, 4, 700, 64), (1, 2, 385, 128),
-          (2, 40, 900, 64), (3, 20, 400, 128)]  # (more chunks than a CTA per SM takes at once)
+          (2, 40, 900, 64), (3, 20, 400, 128),  # (more chunks than a CTA per SM takes at once)
+          (1, 1, 1700, 64), (1, 2, 1500, 128)]  # (few and long: walked in segments)
 
 
 @pytest.mark.parametrize("form", ["plain", "masked", "docs", "init"])
