@@ -775,32 +775,31 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
 struct GatedMaps {
   CUtensorMap q, k, v, o, dq, dk, dv;
 };
-template <int D> constexpr int bwd_threads() { return 4 * D; }
+constexpr int kBwd128Threads = 512;
 constexpr int kBwdAhead = 148;  // units: a CTA on each SM
-template <int D> constexpr size_t bwd_tc_smem() { return 1024 + 4 * (D / 64) * kTileBytes + 2 * (D / 64) * (D / 64) * kStateTile; }
+constexpr size_t kBwd128Smem = 1024 + 4 * 2 * kTileBytes + 2 * 4 * kStateTile;
 
-// Backward of one chunk: dq, dk, dv and dg from q, k, v, dO and the two states, each read once; grid = B*H * chunks.
+// Backward of one chunk at head dim 128: dq, dk, dv and dg from q, k, v, dO and the two states, each read once; grid = B*H * chunks.
 //     E  = dO V^T  (t, s)    dq = e^(G_t) dO S^T        + (E D) K
 //     E' = V dO^T  (s, t)    dk = e^(G_last-G_s) V R^T  + (E' D) Q
 //     P' = K Q^T   (s, t)    dv = e^(G_last-G_s) K R    + (P' D) dO
 // E and its transpose are both computed: an A operand from TMEM cannot be transposed, and two products of 128 x 128 x D cost less
-// than a 32 KB tile through shared memory.  Two score buffers X and Y in TMEM; every pass is scores -> decayed 16-bit scores in
-// place -> the state's part into the accumulator (D 64: the buffer's other half), read and scaled in fp32 -> scores times rows.  The
-// passes are interleaved so that the MMAs of one run under the register work of another:
-//     E X, E' Y | decay X | state X | decay Y | state Y | rows X | rows Y | dq out, P' X | decay X, dk out | state X | rows X | dv out
-// Results are staged over the tile that has no reader left: dq over V, dk over Q, dv over K.
+// than a 32 KB tile through shared memory.  Two buffers X and Y in TMEM of 128 columns of scores and 128 of accumulator; every pass is
+// scores and state's part (MMA) -> decayed 16-bit scores in place, the state's part read and scaled in fp32 -> scores times rows:
+//     E X, E' Y and their states | decay X | decay Y, rows X | rows Y | dq out, P' X and its state | decay X, dk out | rows X | dv out
+// Results are staged over the tile that has no reader left: dq over V, dk over Q, dv over K.  The tiles and states fill the SM's
+// shared memory, so that a CTA's loads overlap nothing but the set-up; the CTA after it finds its tiles in L2.
 // With k.dk split into what the chunk itself contributes and what lies across its end,
 //     dg_t = sum_{u>=t} (q_u.dq_u - (k_u.dk_u)_within) + sum_{s<t} (k_s.dk_s)_across + A <S, R>
 // counts the pairs that cross t and no others, but for those within the chunk, which are the same rounded products in q.dq and in
 // k.dk and cancel.  (gated_simt.cuh has <S', R> for the last two terms; with operands of 16 bits that would leave the roundings of all
 // pairs across the chunk's end at every position.)
-//   warp w: rows 32 (w % 4) .., group w / 4 of D / 32: 4096 / D columns of the scores and 32 of the accumulator
-template <typename T, int D>
-__global__ void __launch_bounds__(bwd_threads<D>(), D == 64 ? 2 : 1)
-gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a) {
+//   warp w: rows 32 (w % 4) .., columns 32 (w / 4) .. of the scores and of the accumulator
+template <typename T>
+__global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a) {
   using namespace ptx;
-  constexpr int NT = D / 64, NG = D / 32, NB = 4 / NG;  // column groups; 32-column blocks of the scores per warp
-  constexpr uint32_t kCols = D == 64 ? 256 : 512, kBuf = kCols / 2, kAccAt = D == 64 ? 64 : 128;
+  constexpr int D = 128, NT = 2, NG = 4;  // 64-column panels, 32-column groups
+  constexpr uint32_t kCols = 512, kBuf = 256, kAccAt = 128;
   constexpr bool BF = Pack2<T>::kBf16;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -875,7 +874,7 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
   }
   const bool kp = !a.keep || (c0 + row < a.N && a.keep[b * a.N + c0 + row]);
   __syncthreads();
-  for (int e = tid; e < 4 * kGtChunk; e += bwd_threads<D>()) {
+  for (int e = tid; e < 4 * kGtChunk; e += kBwd128Threads) {
     col_factor<true>(sLow, sG, e >> 7, e & 127);
     col_factor<false>(sUp, sG, e >> 7, e & 127);
   }
@@ -936,46 +935,40 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
     tc_fence_after_sync();
   };
   const uint32_t my_scores = lane_base, my_acc = lane_base + kAccAt + 32 * cg;
-  auto put_scores = [&](uint32_t t, const uint32_t (&pk)[NB][16]) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) tmem_st_x16(t + lane_base + 16 * (NB * cg + i), pk[i]);
+  auto put_scores = [&](uint32_t t, const uint32_t (&pk)[16]) {
+    tmem_st_x16(t + lane_base + 16 * cg, pk);
     tmem_st_wait();
   };
   issue(true, [&] {
     scores(tX, dO, dV, &bar_score[0]);
     scores(tY, dV, dO, &bar_score[1]);
+    if (with_S) times_state_t(tX, dO, sS, &bar_state[0]);
+    if (with_R) times_state_t(tY, dV, sR, &bar_state[1]);
   });
   const float Gr = sG[row], total = sG[kGtChunk - 1];
   const float head = ex2(Gr), tail = ex2(total - Gr);
   const float row_low = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = ex2(sG[32 * wq + 31] - Gr);
   const int panel = cg / 2 * kTileBytes, j0 = 4 * (cg & 1);  // where this thread's 32 columns are in a row of D
 
-  uint32_t pk[NB][16];
+  uint32_t pk[16];
   float ax[32], ay[32];
-  // ---- dq: decayed scores X
-  wait(&bar_score[0]);
-#pragma unroll
-  for (int i = 0; i < NB; ++i) decay_block<T, true>(pk[i], tX + my_scores, NB * cg + i, wq, lane, Gr, row_low, sG, sLow[wq]);
-  sync();
-  issue(with_S, [&] { times_state_t(tX, dO, sS, &bar_state[0]); });
-  put_scores(tX, pk);
-  // ---- dk: decayed scores Y
-  wait(&bar_score[1]);
-#pragma unroll
-  for (int i = 0; i < NB; ++i) decay_block<T, false>(pk[i], tY + my_scores, NB * cg + i, wq, lane, Gr, row_up, sG, sUp[wq]);
-  sync();
-  issue(with_R, [&] { times_state_t(tY, dV, sR, &bar_state[1]); });
-  put_scores(tY, pk);
-  // ---- dq: the state's part, then the rows
 #pragma unroll
   for (int j = 0; j < 32; ++j) ax[j] = 0.f, ay[j] = 0.f;
+  // ---- dq: decayed scores X (packed over what the other warps of the rows have read), the state's part
+  wait(&bar_score[0]);
+  decay_block<T, true>(pk, tX + my_scores, cg, wq, lane, Gr, row_low, sG, sLow[wq]);
+  sync();
+  put_scores(tX, pk);
   if (with_S) {
     wait(&bar_state[0]);
     acc_scaled(ax, tX + my_acc, head);
   }
+  // ---- dk: the same in Y
+  wait(&bar_score[1]);
+  decay_block<T, false>(pk, tY + my_scores, cg, wq, lane, Gr, row_up, sG, sUp[wq]);
   sync();
   issue(true, [&] { times_rows(tX, sK, &bar_rows[0]); });
-  // ---- dk: the same
+  put_scores(tY, pk);
   if (with_R) {
     wait(&bar_state[1]);
     acc_scaled(ay, tY + my_acc, tail);
@@ -988,7 +981,7 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
   if (with_S && with_R) {
     const uint4 *s4 = reinterpret_cast<const uint4*>(sS), *r4 = reinterpret_cast<const uint4*>(sR);
 #pragma unroll 2
-    for (int e = tid; e < NT * NT * kStateTile / 16; e += bwd_threads<D>()) {
+    for (int e = tid; e < NT * NT * kStateTile / 16; e += kBwd128Threads) {
       const uint4 x = s4[e], y = r4[e];
       const uint32_t u[4] = {x.x, x.y, x.z, x.w}, w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -1010,16 +1003,15 @@ gated_bwd_tc_kernel(const __grid_constant__ GatedMaps m, const GatedChunkArgs a)
   sync();
   issue(true, [&] {
     scores(tX, dK, dQ, &bar_score[2]);
+    if (with_R) times_state(tX, dK, sR, &bar_state[2]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) tma_store_tile_x(&m.dq, sV + i * kTileBytes, 64 * i, c0, h, bi);
     tma_store_commit();
   });
   // ---- dv: decayed scores X
   wait(&bar_score[2]);
-#pragma unroll
-  for (int i = 0; i < NB; ++i) decay_block<T, false>(pk[i], tX + my_scores, NB * cg + i, wq, lane, Gr, row_up, sG, sUp[wq]);
+  decay_block<T, false>(pk, tX + my_scores, cg, wq, lane, Gr, row_up, sG, sUp[wq]);
   sync();
-  issue(with_R, [&] { times_state(tX, dK, sR, &bar_state[2]); });
   put_scores(tX, pk);
   // ---- dk out
   wait(&bar_rows[1]);

@@ -124,11 +124,11 @@ int run_tc_bwd(const GatedArgs& g, const void* states, void* ws, int B, int dtyp
     auto kern = gated_bwd64_kernel<T>;
     COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwd64Smem));
     COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)(c.units < kSms ? c.units : kSms)), kBwd64Threads, kBwd64Smem, stream, m, c));
-    return COTT_OK;
+  } else {
+    auto kern = gated_bwd128_kernel<T>;
+    COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwd128Smem));
+    COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)c.units), kBwd128Threads, kBwd128Smem, stream, m, c));
   }
-  auto kern = gated_bwd_tc_kernel<T, D>;
-  COTT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bwd_tc_smem<D>()));
-  COTT_CUDA_TRY(launch_pdl(kern, dim3((unsigned)c.units), bwd_threads<D>(), bwd_tc_smem<D>(), stream, m, c));
   return COTT_OK;
 }
 
