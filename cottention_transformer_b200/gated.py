@@ -138,7 +138,8 @@ def gated_scan(q, k, v, log_decay, keep=None, initial_state=None, return_state=F
 
     Differentiable once in q, k, v, log_decay and initial_state (``return_state`` included).  A gate of ``-inf`` and the first gate of
     a sequence without an initial state have no gradient.  16-bit tensors: the gradient of log_decay carries the roundings of the
-    16-bit products, also where log_decay is float32."""
+    16-bit products, also where log_decay is float32.  float16: a state entry beyond 65504 overflows, and what is smaller than the
+    type's smallest step (weights of less than 2^-24 within 128 positions) is lost."""
     m = _binding.autograd()
     if m is not None:
         r = m.gated_scan(q, k, v, log_decay, keep, initial_state, bool(return_state))
@@ -170,6 +171,7 @@ def gated_scan_step(state, q, k, v, log_decay):
                                         _layout(q, k, v, out, log_decay), B, H, T, D, _lib.DTYPE_CODE[q.dtype], _lib.DTYPE_CODE[log_decay.dtype],
                                         _lib.stream_ptr(q.device))
     _lib.check(st, "cott_gated_step")
+    torch.autograd.graph.increment_version(state)
     return out
 
 

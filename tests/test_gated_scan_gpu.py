@@ -300,6 +300,84 @@ def test_a_saved_graph_can_be_walked_twice_and_not_differentiated_again():
         torch.autograd.grad(c[0].sum(), q)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_decay_per_head(dtype, D):
+    """A fixed decay as an expanded view: its gradient is the sum over batch and positions."""
+    from cottention_transformer_b200 import gated_scan
+    q, k, v, g, keep, st, do, dst = _inputs(2, 3, 200, D, dtype, seed=30)
+    d = torch.tensor([-0.5, -0.05, -0.01]).to(dtype)
+    want = _truth(q, k, v, d.view(1, 3, 1).expand(2, 3, 200).contiguous(), None, None, do, None)
+    leaf = d.cuda().requires_grad_()
+    out = gated_scan(q.cuda(), k.cuda(), v.cuda(), leaf.view(1, 3, 1).expand(2, 3, 200))
+    assert O.rel(out, want[0]) <= _tol("out", dtype)
+    got, = torch.autograd.grad(out, leaf, do.cuda())
+    # a sum of 400 terms, each rounded to the type by the operator (u) and with its own error (6 u) in the 2-norm
+    err = (got.double().cpu() - want[5].sum((0, 2))).abs()
+    assert (err <= 7 * _tol("dg", dtype) * want[5].norm(dim=2).sum(0) + 2 * _u(dtype) * want[5].sum((0, 2)).abs() + 1e-5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_one_result_alone(dtype):
+    """The initial state's gradient where the last state is not asked for, and gradients through the last state alone."""
+    from cottention_transformer_b200 import gated_scan
+    q, k, v, g, keep, st, do, dst = _inputs(1, 2, 300, 64, dtype, seed=31, init=True)
+    want = _truth(q, k, v, g, None, st, do, None)
+    leaf = [t.cuda().requires_grad_() for t in (q, k, v, g, st)]
+    out = gated_scan(*leaf[:4], initial_state=leaf[4])
+    for name, a, b in zip(NAMES[2:], torch.autograd.grad(out, leaf, do.cuda()), want[2:]):
+        assert O.rel(a, b) <= _tol(name, dtype), name
+    want = _truth(q, k, v, g, None, st, torch.zeros_like(do), dst)
+    state = gated_scan(*leaf[:4], initial_state=leaf[4], return_state=True)[1]
+    for name, a, b in zip(NAMES[2:], torch.autograd.grad(state, leaf, dst.cuda()), want[2:]):
+        assert O.rel(a, b) <= 2 * _tol(name, dtype), name
+
+
+def test_calls_on_two_streams_at_once():
+    from cottention_transformer_b200 import gated_scan
+    xs = [[t.cuda() for t in (*_inputs(2, 4, 1000, 64, torch.bfloat16, seed=s)[:4], _inputs(2, 4, 1000, 64, torch.bfloat16, seed=s)[6])] for s in (32, 33)]
+
+    def train(x):
+        leaf = [t.detach().requires_grad_() for t in x[:4]]
+        out = gated_scan(*leaf)
+        return out, *torch.autograd.grad(out, leaf, x[4])
+
+    want = [train(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(5):
+        for i, (stream, x) in enumerate(zip(streams, xs)):
+            with torch.cuda.stream(stream):
+                got[i].append(train(x))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        for r in rs:
+            assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+def test_rows_past_the_sequences_are_left_alone():
+    """Outputs and states written through a view of a larger buffer: nothing beside it changes."""
+    from cottention_transformer_b200 import _lib
+    import ctypes
+    L = _lib.lib()
+    B, H, N, D = 2, 2, 150, 64
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v, g, *_ = (t if t is None else t.cuda() for t in _inputs(B, H, N, D, dtype, seed=34))
+        code = _lib.DTYPE_CODE[dtype]
+        big = torch.full((B, H, N + 40, D), 7.0, dtype=dtype, device="cuda")
+        states = torch.empty(L.cott_gated_scan_states_bytes(B, H, N, D, code), dtype=torch.uint8, device="cuda")
+        ws = torch.empty(max(L.cott_gated_scan_workspace_bytes(B, H, N, D, code, 0), 16), dtype=torch.uint8, device="cuda")
+        lay = _lib.CottGatedLayout()
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", big), ("gate", g)):
+            setattr(lay, name, _lib.CottStrides(*t.stride()[:3]))
+        _lib.check(L.cott_gated_scan_fwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(g), None, None, _lib.ptr(big), None, _lib.ptr(states),
+                                         _lib.ptr(ws), ctypes.byref(lay), B, H, N, D, code, code, _lib.stream_ptr(q.device)), "cott_gated_scan_fwd")
+        from cottention_transformer_b200 import gated_scan
+        assert torch.equal(big[:, :, :N], gated_scan(q, k, v, g)) and (big[:, :, N:] == 7).all()
+        _lib.check_device_status()
+
+
 def test_empty_sequences():
     from cottention_transformer_b200 import gated_scan, gated_scan_step
     q = torch.empty(2, 3, 0, 64, device="cuda", requires_grad=True)
