@@ -1085,7 +1085,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     else
       static_cast<T*>(a.dgate)[o] = from_acc<T>(x);
   }
-  issue(true, [&] { tma_store_wait_read<0>(); });
+  if (warp == 0) tma_store_wait_read<0>();  // (by all lanes: the groups belong to the one that stored)
 }
 
 // ---- backward at head dim 64: a persistent kernel ------------------------------------------------------------------------
