@@ -373,7 +373,7 @@ __device__ __forceinline__ void gated_chunk(const GatedArgs& g, float* sA, float
 
 // FWD: grid = B*H * chunks.  Backward: grid = (B*H * chunks, 3), y = dq, dk, dv.
 template <typename T, int D, bool FWD>
-__global__ void __launch_bounds__(kGsThreads, D > 64 ? 1 : 2) gated_chunk_kernel(const GatedArgs g) {
+__global__ void __launch_bounds__(kGsThreads, D > 64 ? 1 : 3) gated_chunk_kernel(const GatedArgs g) {
   extern __shared__ __align__(16) unsigned char gs_smem[];
   float* sA = reinterpret_cast<float*>(gs_smem);
   float* sB = sA + kGsChunk * (D + 4);
@@ -408,6 +408,7 @@ __global__ void __launch_bounds__(kGsThreads) gated_dgate_kernel(const GatedArgs
   double cross = 0.0;
   if (chunk + 1 < g.nchunks || g.dfinal) {
     const float *S = g.prefix + (bh * (g.nchunks + 1) + chunk + 1) * static_cast<long>(D * D), *R = g.suffix + (bh * g.nchunks + chunk) * static_cast<long>(D * D);
+#pragma unroll 8
     for (int e = tid; e < D * D; e += kGsThreads) cross = fma(static_cast<double>(S[e]), static_cast<double>(R[e]), cross);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) cross += __shfl_xor_sync(0xffffffffu, cross, off);
