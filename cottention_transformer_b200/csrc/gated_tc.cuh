@@ -1099,21 +1099,27 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
 //   warps 24-27: gates of the next chunk, masked rows, <S, R>, dg     warp 28: TMA loads
 //   warps 29-31, one thread each: the MMAs and the stores of a pass, so that the scores of the next chunk are under way while the
 //   last rows of this one are written, and no working warp spends its time on issuing
-// Two stages of (dO, V, K, Q, S, R), 80 KB; 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and
-// 32 of the accumulator; 64 each for the state's part of dq and dk.
-// A result is staged over a tile when the MMAs that read it have completed, whichever group issued them; the barriers for that are
-// kept per stage, so that nobody can be a whole phase ahead of one that is still waiting.
+// Two stages of (dO, V, K, Q, S, R), 80 KB, and a tile per group for its results, so that a stage is free as soon as the last group
+// has its products (staged over the tiles instead, a stage was held until the stores had been read, 2000 cycles of a chunk's
+// 8000); 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
+// state's part of dq and dk.
+// Barriers that a stage's chunk completes once are kept per stage, so that nobody can be a whole phase ahead of one that waits.
 // Every wait is bounded.  After one that gave up every further wait returns at once; the warps that share a named barrier go through
 // all of them all the same.
 constexpr int kBwd64Threads = 1024;
 constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
-constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage;
+constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage + 3 * kTileBytes;
 
 struct __align__(16) BwdInfo {  // of a chunk: one more than there are stages, so that a chunk's is made before its tiles arrive
-  float G[kGtChunk], low[4][kGtChunk], up[4][kGtChunk];
+  float G[kGtChunk], gate[kGtChunk];
+  float low[192], up[192];  // column factors of row blocks 1, 2, 3 (32, 64, 96 columns) and 0, 1, 2 (96, 64, 32 columns)
   int has_s, has_r;
-  float gate[kGtChunk], qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];  // (the dot products by halves)
 };
+struct BwdDots {  // a stage's dot products, by halves of the columns
+  float qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];
+};
+__device__ __forceinline__ int low_at(int w) { return 16 * w * (w - 1); }                      // of column 0 of row block w
+__device__ __forceinline__ int up_at(int w) { return (w == 0 ? 0 : w == 1 ? 96 : 160) - 32 * (w + 1); }
 
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
@@ -1124,8 +1130,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ BwdInfo info[3];
-  __shared__ uint64_t bar_full[2], bar_free[2], bar_ready[2], bar_dots[2], bar_score[3][2], bar_state[3][2], bar_rows[3][2];
-  __shared__ uint64_t bar_packed[3], bar_scaled, bar_read[3], bar_staged[3];  // a group to its issuing thread, once per chunk each
+  __shared__ BwdDots dots[2];
+  __shared__ uint64_t bar_full[2], bar_free[2], bar_ready[2], bar_dots[2], bar_state[2], bar_score[3][2], bar_rows[3][2];
+  __shared__ uint64_t bar_packed[3], bar_scaled, bar_read[3], bar_staged[3], bar_stored[3];  // a group to its issuing thread, once per chunk each
   __shared__ uint32_t tmem_slot;
   __shared__ float sPart[12];
   __shared__ int abort_flag_s, loads_s;
@@ -1146,12 +1153,12 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar_full[s], 1);
-      mbar_init(&bar_free[s], 7);   // three stores, four warps that took <S, R>
+      mbar_init(&bar_free[s], 28);  // the warps of the passes, four that took <S, R>
       mbar_init(&bar_ready[s], 4);
       mbar_init(&bar_dots[s], 16);
+      mbar_init(&bar_state[s], 1);  // of dv
       for (int p = 0; p < 3; ++p) {
         mbar_init(&bar_score[p][s], 1);
-        mbar_init(&bar_state[p][s], 1);
         mbar_init(&bar_rows[p][s], 1);
       }
     }
@@ -1160,6 +1167,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       mbar_init(&bar_packed[p], 8);
       mbar_init(&bar_read[p], 8);
       mbar_init(&bar_staged[p], 8);
+      mbar_init(&bar_stored[p], 1);
     }
     mbar_fence_init();
     abort_flag_s = 0;
@@ -1180,12 +1188,13 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   pdl_wait_prior();
   const uint32_t tmem = tmem_slot;
 
-  // E = dO V^T    E' = V dO^T    P' = K Q^T        rows of: K, Q, dO       result over: Q, K, V
+  // E = dO V^T    E' = V dO^T    P' = K Q^T        rows of: K, Q, dO
   auto tile_of = [&](int s, int which) { return smem + s * kBwd64Stage + which * kTileBytes; };  // O 0, V 1, K 2, Q 3
   auto tile_a = [&](int s, int pass) { return tile_of(s, pass); };
   auto tile_b = [&](int s, int pass) { return tile_of(s, pass == 0 ? 1 : pass == 1 ? 0 : 3); };
   auto tile_c = [&](int s, int pass) { return tile_of(s, pass == 0 ? 2 : pass == 1 ? 3 : 0); };
-  auto tile_out = [&](int s, int pass) { return tile_of(s, 3 - pass); };
+  auto tile_x = [&](int s, int pass) { return tile_of(s, 3 - pass); };  // the rows that dq, dk are multiplied with: Q, K
+  auto tile_out = [&](int pass) { return smem + 2 * kBwd64Stage + pass * kTileBytes; };
 
   if (warp >= 29) {
     // ---------------------------------------------------------------- MMAs and stores of a pass
@@ -1195,13 +1204,13 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
                          kIdescM = make_idesc(128, 32, BF, false, true);
       const uint32_t tP = tmem + 128 * pass;
       const CUtensorMap* out = pass == 0 ? &m.dq : pass == 1 ? &m.dk : &m.dv;
-      auto store = [&](long unit, int n) {  // the result of the n-th chunk; its stage is free when it has been read
+      auto store = [&](long unit, int n) {  // the result of the n-th chunk
         if (!wait_bar1(&bar_staged[pass], n & 1, abort_flag, kWaitAcc, n)) return false;
         const long bh = unit / a.nchunks;
-        tma_store_tile(out, tile_out(n & 1, pass), static_cast<int>(unit % a.nchunks) * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
+        tma_store_tile(out, tile_out(pass), static_cast<int>(unit % a.nchunks) * kGtChunk, static_cast<int>(bh % a.H), static_cast<int>(bh / a.H));
         tma_store_commit();
         tma_store_wait_read<0>();
-        mbar_arrive(&bar_free[n & 1]);
+        mbar_arrive(&bar_stored[pass]);
         return true;
       };
       int n = 0;
@@ -1216,15 +1225,10 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_ss(tP, dA + 2 * k, dB + 2 * k, kIdescP, k > 0);
         mma_commit(&bar_score[pass][s]);
-        if (pass < 2) {
-          if (with_state) {
-            const uint64_t d = kdesc(smem_u32(pass == 0 ? state_s(s) : state_r(s)));
+        if (pass < 2 && with_state) {  // (complete when the rows are: the same thread commits them)
+          const uint64_t d = kdesc(smem_u32(pass == 0 ? state_s(s) : state_r(s)));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ss(tmem + 384 + 64 * pass, dA + 2 * k, d + 2 * k, kIdescK, k > 0);
-            mma_commit(&bar_state[pass][s]);
-          } else {
-            mbar_arrive(&bar_state[pass][s]);  // (one phase per chunk, whether there is a state or not; bar_scaled likewise)
-          }
+          for (int k = 0; k < 4; ++k) mma_ss(tmem + 384 + 64 * pass, dA + 2 * k, d + 2 * k, kIdescK, k > 0);
         }
         if (n > 0 && !(ok = store(unit - gridDim.x, n - 1))) break;
         if (!(ok = wait_bar1(&bar_packed[pass], n & 1, abort_flag, kWaitScoreReady, n))) break;
@@ -1236,9 +1240,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
             for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
               for (int k = 0; k < 4; ++k) mma_ss(tP + 64 * hh + 32, dA + 2 * k, d + 4 * hh + 128 * k, kIdescM, k > 0);
-            mma_commit(&bar_state[2][s]);
+            mma_commit(&bar_state[s]);
           } else {
-            mbar_arrive(&bar_state[2][s]);
+            mbar_arrive(&bar_state[s]);  // (one phase per chunk, whether there is a state or not; bar_scaled likewise)
           }
           if (!(ok = wait_bar1(&bar_scaled, n & 1, abort_flag, kWaitScoreReady, n))) break;
           tc_fence_after_sync();
@@ -1271,6 +1275,15 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         if (has_s(chunk)) bulk_load(state_s(s), a.S + unit * kStateTile, kStateTile, &bar_full[s]);
         if (has_r(chunk)) bulk_load(state_r(s), a.R + unit * kStateTile, kStateTile, &bar_full[s]);
         loads_s = n + 1;
+        const long next = unit + 2 * static_cast<long>(gridDim.x);  // the chunk that this stage takes next, into L2
+        if (next < a.units) {
+          const long nbh = next / a.nchunks;
+          const int ny = static_cast<int>(next % a.nchunks) * kGtChunk, nh = static_cast<int>(nbh % a.H), nb = static_cast<int>(nbh / a.H);
+          tma_prefetch_tile(&m.o, ny, nh, nb);
+          tma_prefetch_tile(&m.v, ny, nh, nb);
+          tma_prefetch_tile(&m.k, ny, nh, nb);
+          tma_prefetch_tile(&m.q, ny, nh, nb);
+        }
       }
     }
   } else if (warp >= 24) {
@@ -1299,9 +1312,9 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       if (t == 0) f.has_s = has_s(chunk), f.has_r = has_r(chunk);
       named_sync(4, 128);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        col_factor<true>(f.low, f.G, w, t);
-        col_factor<false>(f.up, f.G, w, t);
+      for (int w = 0; w < 3; ++w) {
+        if (t < 32 * w + 32) f.low[low_at(w + 1) + t] = ex2(f.G[32 * w + 31] - f.G[t]);
+        if (t >= 32 * w + 32) f.up[up_at(w) + t] = ex2(f.G[t] - f.G[32 * w + 31]);
       }
     };
     // dg of a chunk that is done (unit u, the n-th of this CTA): its dot products, <S, R> as this warp's part
@@ -1310,11 +1323,12 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       wait_bar_warp(&bar_dots[n & 1], (n >> 1) & 1, abort_flag, kWaitAcc, n);
       const long bh = u / a.nchunks, b = bh / a.H;
       const int chunk = static_cast<int>(u % a.nchunks), h = static_cast<int>(bh % a.H), pos = chunk * kGtChunk + t;
-      float run = (f.qd[0][t] + f.qd[1][t]) - (f.kd[0][t] + f.kd[1][t]), up = f.bd[0][t] + f.bd[1][t];
+      const BwdDots& d = dots[n & 1];
+      float run = (d.qd[0][t] + d.qd[1][t]) - (d.kd[0][t] + d.kd[1][t]), up = d.bd[0][t] + d.bd[1][t];
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {  // run: from the row to the warp's end; up: to the row
-        const float d = __shfl_down_sync(0xffffffffu, run, off), x = __shfl_up_sync(0xffffffffu, up, off);
-        if (lane + off < 32) run += d;
+        const float r = __shfl_down_sync(0xffffffffu, run, off), x = __shfl_up_sync(0xffffffffu, up, off);
+        if (lane + off < 32) run += r;
         if (lane >= off) up += x;
       }
       named_sync(4, 128);  // (the sums of the chunk before have been read)
@@ -1408,15 +1422,15 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     int n = 0;
     for (long unit = blockIdx.x; unit < a.units; unit += gridDim.x, ++n) {
       const int s = n & 1;
-      BwdInfo& f = info[n % 3];
-      unsigned char* sOut = tile_out(s, pass);
+      const BwdInfo& f = info[n % 3];
+      unsigned char *sX = tile_x(s, pass), *sOut = tile_out(pass);
       // (tiles are read row by row below: every reader has to see the loads' completion itself)
       if (!wait(n, &bar_full[s], &bar_ready[s], &bar_score[pass][s])) break;
       tc_fence_after_sync();
       const bool with_state = lower ? f.has_s : f.has_r;
       const float Gr = f.G[row], signedG = sign * Gr;
       const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
-      const float* col = lower ? f.low[wq] : f.up[wq];
+      const float* col = lower ? f.low + low_at(wq) : f.up + up_at(wq);  // (of a block without factors: not read)
       // decayed, masked, packed in place: the half's first 32 columns into its first 16, then the others into the next 16
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
@@ -1461,7 +1475,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
       if (pass == 2) {
         if (with_state) {  // dv: the state's part, scaled where it is
-          if (!wait(n, &bar_state[2][s])) break;
+          if (!wait(n, &bar_state[s])) break;
           tc_fence_after_sync();
           uint32_t r[32];
           tmem_ld_x32(tMine + 32, r);
@@ -1477,22 +1491,28 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         }
         warp_arrive(&bar_scaled, lane);
       }
-      // the rows, and the other groups' MMAs that read the tile under the result
-      if (!(pass == 0   ? wait(n, &bar_rows[0][s], &bar_score[2][s], &bar_rows[1][s])
-            : pass == 1 ? wait(n, &bar_rows[1][s], &bar_score[2][s], &bar_rows[0][s], &bar_state[2][s])
-                        : wait(n, &bar_rows[2][s], &bar_score[0][s], &bar_score[1][s], &bar_state[1][s])))
+      // the rows; and the place of the result: what was there has been stored
+      bool ok = false;
+      for (uint32_t i = 0; i < kMaxPolls && !ok; ++i) {
+        const bool d0 = mbar_try_wait(&bar_rows[pass][s], (n >> 1) & 1), d1 = n == 0 || mbar_try_wait(&bar_stored[pass], (n - 1) & 1);
+        ok = __all_sync(0xffffffffu, d0 && d1);
+        if (!ok && *abort_flag) break;
+      }
+      if (!ok) {
+        if (!*abort_flag) atomicCAS(&g_cott_status, 0, (kWaitChunkMma << 16) | (n & 0xffff));
+        *abort_flag = 1;
         break;
+      }
       tc_fence_after_sync();
-      // q.dq, k.dk over the half's columns (k.dk by parts); the result's row takes the place of q's, k's
+      // the result's row, and q.dq, k.dk over the half's columns (k.dk by parts)
       float2 dot = make_float2(0.f, 0.f), across = make_float2(0.f, 0.f);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        uint4 *p0 = tile_piece(sOut, row, 4 * half + 2 * i), *p1 = tile_piece(sOut, row, 4 * half + 2 * i + 1);
         uint32_t x[16];
         tmem_ld_x16(tMine + 32 + 16 * i, x);
         uint4 u, w;
         if (pass < 2) {
-          u = *p0, w = *p1;
+          u = *tile_piece(sX, row, 4 * half + 2 * i), w = *tile_piece(sX, row, 4 * half + 2 * i + 1);
           uint32_t y[16];
           if (with_state) tmem_ld_x16(tState + 16 * i, y);
           tmem_ld_wait();
@@ -1517,17 +1537,18 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         u.z = Pack2<T>::pack(__uint_as_float(x[4]), __uint_as_float(x[5])), u.w = Pack2<T>::pack(__uint_as_float(x[6]), __uint_as_float(x[7]));
         w.x = Pack2<T>::pack(__uint_as_float(x[8]), __uint_as_float(x[9])), w.y = Pack2<T>::pack(__uint_as_float(x[10]), __uint_as_float(x[11]));
         w.z = Pack2<T>::pack(__uint_as_float(x[12]), __uint_as_float(x[13])), w.w = Pack2<T>::pack(__uint_as_float(x[14]), __uint_as_float(x[15]));
-        *p0 = u;
-        *p1 = w;
+        *tile_piece(sOut, row, 4 * half + 2 * i) = u;
+        *tile_piece(sOut, row, 4 * half + 2 * i + 1) = w;
       }
       fence_proxy_async_smem();
       warp_arrive(&bar_staged[pass], lane);
+      if (lane == 0) mbar_arrive(&bar_free[s]);  // (all MMAs of this pass that read the stage have completed, and its rows have been read)
       if (pass < 2) {
         if (pass == 0) {
-          f.qd[half][row] = dot.x + dot.y;
+          dots[s].qd[half][row] = dot.x + dot.y;
         } else {
-          f.kd[half][row] = dot.x + dot.y;
-          f.bd[half][row] = scale * (across.x + across.y);
+          dots[s].kd[half][row] = dot.x + dot.y;
+          dots[s].bd[half][row] = scale * (across.x + across.y);
         }
         warp_arrive(&bar_dots[s], lane);
       }
