@@ -1275,15 +1275,6 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
         if (has_s(chunk)) bulk_load(state_s(s), a.S + unit * kStateTile, kStateTile, &bar_full[s]);
         if (has_r(chunk)) bulk_load(state_r(s), a.R + unit * kStateTile, kStateTile, &bar_full[s]);
         loads_s = n + 1;
-        const long next = unit + 2 * static_cast<long>(gridDim.x);  // the chunk that this stage takes next, into L2
-        if (next < a.units) {
-          const long nbh = next / a.nchunks;
-          const int ny = static_cast<int>(next % a.nchunks) * kGtChunk, nh = static_cast<int>(nbh % a.H), nb = static_cast<int>(nbh / a.H);
-          tma_prefetch_tile(&m.o, ny, nh, nb);
-          tma_prefetch_tile(&m.v, ny, nh, nb);
-          tma_prefetch_tile(&m.k, ny, nh, nb);
-          tma_prefetch_tile(&m.q, ny, nh, nb);
-        }
       }
     }
   } else if (warp >= 24) {
