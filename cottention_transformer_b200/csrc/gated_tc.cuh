@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char *sQ = smem, *sK = sQ + NT * kTileBytes, *sV = sK + NT * kTileBytes, *sO = sV + NT * kTileBytes, *sS = sO + NT * kTileBytes,
                 *sR = sS + NT * NT * kStateTile;
-  __shared__ uint64_t bar_full, bar_score[3], bar_state[3], bar_rows[3];
+  __shared__ uint64_t bar_full[3], bar_score[3], bar_state[3], bar_rows[3];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
   __shared__ __align__(16) float sG[kGtChunk], sLow[4][kGtChunk], sUp[4][kGtChunk];
@@ -820,8 +820,8 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   const bool with_S = chunk > 0 || a.with_first, with_R = chunk + 1 < a.nchunks || a.with_last;
   const uint32_t lane_base = static_cast<uint32_t>(32 * wq) << 16;
   if (tid == 0) {
-    mbar_init(&bar_full, 1);
     for (int i = 0; i < 3; ++i) {
+      mbar_init(&bar_full[i], 1);  // dO and V; the states; K and Q
       mbar_init(&bar_score[i], 1);
       mbar_init(&bar_state[i], 1);
       mbar_init(&bar_rows[i], 1);
@@ -845,16 +845,20 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   const uint32_t tX = tmem_slot, tY = tX + kBuf;
   if (warp == 0) {
     if (elect_one()) {
-      mbar_expect_tx(&bar_full, 4 * NT * kTileBytes + ((with_S ? 1 : 0) + (with_R ? 1 : 0)) * NT * NT * kStateTile);
+      for (int i = 0; i < 3; i += 2) mbar_expect_tx(&bar_full[i], 2 * NT * kTileBytes);
+      mbar_expect_tx(&bar_full[1], ((with_S ? 1 : 0) + (with_R ? 1 : 0)) * NT * NT * kStateTile);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        tma_load_tile_x(sO + i * kTileBytes, &m.o, &bar_full, 64 * i, c0, h, bi);
-        tma_load_tile_x(sV + i * kTileBytes, &m.v, &bar_full, 64 * i, c0, h, bi);
-        tma_load_tile_x(sK + i * kTileBytes, &m.k, &bar_full, 64 * i, c0, h, bi);
-        tma_load_tile_x(sQ + i * kTileBytes, &m.q, &bar_full, 64 * i, c0, h, bi);
+        tma_load_tile_x(sO + i * kTileBytes, &m.o, &bar_full[0], 64 * i, c0, h, bi);
+        tma_load_tile_x(sV + i * kTileBytes, &m.v, &bar_full[0], 64 * i, c0, h, bi);
       }
-      if (with_S) bulk_load(sS, a.S + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
-      if (with_R) bulk_load(sR, a.R + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full);
+      if (with_S) bulk_load(sS, a.S + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full[1]);
+      if (with_R) bulk_load(sR, a.R + unit * (NT * NT * kStateTile), NT * NT * kStateTile, &bar_full[1]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        tma_load_tile_x(sK + i * kTileBytes, &m.k, &bar_full[2], 64 * i, c0, h, bi);
+        tma_load_tile_x(sQ + i * kTileBytes, &m.q, &bar_full[2], 64 * i, c0, h, bi);
+      }
       const long next = unit + kBwdAhead;  // the tiles of the CTA that takes this one's place, into L2
       if (next < a.units) {
         const long nbh = next / a.nchunks;
@@ -878,16 +882,19 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     col_factor<true>(sLow, sG, e >> 7, e & 127);
     col_factor<false>(sUp, sG, e >> 7, e & 127);
   }
-  // (every thread reads rows of the tiles later on, so every thread waits for them)
-  wait_bar_warp(&bar_full, 0, abort_flag, kWaitChunkTma, chunk);
-  if (a.keep) {  // nothing of a masked position gets into a product
-    if (!kp) {
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int j = 0; j < 8; ++j)
-        for (int i = cg; i < 4 * NT; i += NG) *tile_piece(sQ + i * kTileBytes, row, j) = zero;
+  // (every thread reads rows of the tiles later on, so every thread waits for them; nothing of a masked position gets into a product)
+  auto arrived = [&](int which, unsigned char* tiles) {
+    wait_bar_warp(&bar_full[which], 0, abort_flag, kWaitChunkTma, chunk);
+    if (a.keep) {
+      if (!kp) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) *tile_piece(tiles + cg * kTileBytes, row, j) = zero;
+      }
+      fence_proxy_async_smem();
     }
-    fence_proxy_async_smem();
-  }
+  };
+  static_assert(2 * NT == NG);  // (a panel each)
+  arrived(0, sV);
   __syncthreads();
   constexpr uint32_t kIdescP = make_idesc(128, 128, BF, false, false), kIdescK = make_idesc(128, D, BF, false, false), kIdescM = make_idesc(128, D, BF, false, true);
   constexpr uint64_t kPanel = kTileBytes >> 4, kStatePanel = (NT * kStateTile) >> 4;
@@ -942,6 +949,9 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   issue(true, [&] {
     scores(tX, dO, dV, &bar_score[0]);
     scores(tY, dV, dO, &bar_score[1]);
+  });
+  if (warp == 0) wait_bar_warp(&bar_full[1], 0, abort_flag, kWaitChunkTma, chunk);
+  issue(true, [&] {
     if (with_S) times_state_t(tX, dO, sS, &bar_state[0]);
     if (with_R) times_state_t(tY, dV, sR, &bar_state[1]);
   });
@@ -966,6 +976,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   // ---- dk: the same in Y
   wait(&bar_score[1]);
   decay_block<T, false>(pk, tY + my_scores, cg, wq, lane, Gr, row_up, sG, sUp[wq]);
+  arrived(2, sQ);
   sync();
   issue(true, [&] { times_rows(tX, sK, &bar_rows[0]); });
   put_scores(tY, pk);
@@ -979,6 +990,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   sBd[cg][row] = with_R ? row_dot32<T>(sK + panel, row, j0, ay) : 0.f;
   float cross = 0.f;
   if (with_S && with_R) {
+    wait_bar_warp(&bar_full[1], 0, abort_flag, kWaitChunkTma, chunk);
     const uint4 *s4 = reinterpret_cast<const uint4*>(sS), *r4 = reinterpret_cast<const uint4*>(sR);
 #pragma unroll 2
     for (int e = tid; e < NT * NT * kStateTile / 16; e += kBwd128Threads) {
@@ -1068,7 +1080,9 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     for (int i = 0; i < NT; ++i) tma_store_tile_x(&m.dv, sK + i * kTileBytes, 64 * i, c0, h, bi);
     tma_store_commit();
   });
-  if (tid == 0 && *abort_flag) mbar_wait(&bar_full, 0, 64);  // no load may be in flight when the CTA leaves
+  if (tid == 0 && *abort_flag) {  // no load may be in flight when the CTA leaves
+    for (int i = 0; i < 3; ++i) mbar_wait(&bar_full[i], 0, 64);
+  }
   if (warp == 1) tmem_dealloc(tX, kCols);
   if (warp < 4 && c0 + row < a.N && !*abort_flag) {
     float sr = 0.f;
