@@ -378,6 +378,26 @@ def test_rows_past_the_sequences_are_left_alone():
         _lib.check_device_status()
 
 
+@pytest.mark.parametrize("D", [64, 32])
+def test_offsets_past_32_bits(D):
+    """More than 2^31 elements per tensor: the last positions, behind a gate that drops the state, are a sequence of their own."""
+    from cottention_transformer_b200 import gated_scan
+    dtype, N, T = torch.bfloat16, 2 ** 31 // D + 1234, 700
+    if torch.cuda.mem_get_info()[0] < 14 * 2 * N * D:
+        pytest.skip("not enough device memory")
+    r = torch.Generator(device="cuda").manual_seed(35)
+    q, k, v, do = (torch.randn(1, 1, N, D, dtype=dtype, device="cuda", generator=r).mul_(s) for s in (D ** -0.5, D ** -0.5, 1, 1))
+    g = torch.nn.functional.logsigmoid(torch.randn(1, 1, N, device="cuda", generator=r) + 2)
+    g[:, :, N - T] = float("-inf")
+    leaf = [t.requires_grad_() for t in (q, k, v, g)]
+    out = gated_scan(*leaf)
+    got = [t.detach()[:, :, N - T:].cpu() for t in (out, *torch.autograd.grad(out, leaf, do))]
+    x = [t.detach()[:, :, N - T:].cpu() for t in (q, k, v, g)]
+    want = _truth(*x, None, None, do[:, :, N - T:].cpu(), None)
+    for name, a, b in zip(("out", "dq", "dk", "dv", "dg"), got, (want[0], *want[2:])):
+        assert O.rel(a, b) <= _tol(name, dtype), name
+
+
 def test_empty_sequences():
     from cottention_transformer_b200 import gated_scan, gated_scan_step
     q = torch.empty(2, 3, 0, 64, device="cuda", requires_grad=True)

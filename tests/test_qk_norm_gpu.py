@@ -84,6 +84,26 @@ def test_rows_of_zeros_and_of_large_values():
         assert torch.isfinite(a).all() and O.rel(a, b) <= _tol(name, torch.float16, torch.float32), name
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in a packed projection: the last positions against fp64."""
+    from cottention_transformer_b200 import qk_norm_rotary
+    H, D, T, dtype = 16, 64, 50, torch.bfloat16
+    N = 2 ** 31 // (2 * H * D) + 77
+    if torch.cuda.mem_get_info()[0] < 10 * 2 ** 31:
+        pytest.skip("not enough device memory")
+    r = torch.Generator(device="cuda").manual_seed(8)
+    qk = torch.randn(1, N, 2, H, D, dtype=dtype, device="cuda", generator=r).requires_grad_()
+    dq, dk = (torch.randn(1, H, N, D, dtype=dtype, device="cuda", generator=r) for _ in range(2))
+    _, _, qw, kw, tables, _, _ = _inputs(1, 1, 1, N, D, dtype, torch.float32, 32, False, seed=8)
+    a, b = qk_norm_rotary(qk[:, :, 0].transpose(1, 2), qk[:, :, 1].transpose(1, 2), qw.cuda(), kw.cuda(), rotary=tuple(t.cuda() for t in tables))
+    d = torch.autograd.grad((a, b), qk, (dq, dk))[0].detach()[:, N - T:].cpu()
+    tail = lambda t: t.detach()[:, :, N - T:].cpu()  # noqa: E731
+    x = qk.detach()[:, N - T:].cpu()
+    want = _truth(x[:, :, 0].transpose(1, 2), x[:, :, 1].transpose(1, 2), qw, kw, tuple(t[N - T:] for t in tables), tail(dq), tail(dk))
+    for name, s, t in zip(("q", "k", "dq", "dk"), (tail(a), tail(b), d[:, :, 0].transpose(1, 2), d[:, :, 1].transpose(1, 2)), want):
+        assert O.rel(s, t) <= _tol(name, dtype, torch.float32), name
+
+
 def test_unit_weights_give_the_l2_normalisation():
     from cottention_transformer_b200 import qk_norm_rotary
     q = torch.randn(2, 3, 50, 64, device="cuda")
