@@ -5,8 +5,8 @@
 //                       (backwards: R <- A R + Q^T diag(e^(G_t)) dO), and leaves the state before (after) every chunk in memory as
 //                       the 16-bit operand that the other kernel wants.  The weighted operand is split into a 16-bit head and a
 //                       16-bit tail, two MMAs, so that a state is exact to about 2^-17: it lasts for the rest of the sequence.
-//   gated_fwd_tc_kernel, gated_bwd_tc_kernel   one CTA per chunk, none of which waits for another: scores by MMA, decayed, masked and
-//                       rounded to 16 bits in registers, back to TMEM as the A operand of the product with the rows; the state's part in
+//   gated_fwd_tc_kernel, gated_bwd64_kernel, gated_bwd128_kernel   take the chunks, none of which waits for another: scores by MMA,
+//                       decayed, masked and rounded to 16 bits in registers, back to TMEM as the A operand of the product with the rows; the state's part in
 //                       fp32, scaled by the row factor, beside it.
 // HBM-bound: the walk reads two tensors and writes half of one, the chunks read three and half of one, backwards four and a whole.
 //
@@ -788,7 +788,9 @@ constexpr size_t kBwd128Smem = 1024 + 4 * 2 * kTileBytes + 2 * 4 * kStateTile;
 // scores and state's part (MMA) -> decayed 16-bit scores in place, the state's part read and scaled in fp32 -> scores times rows:
 //     E X, E' Y and their states | decay X | decay Y, rows X | rows Y | dq out, P' X and its state | decay X, dk out | rows X | dv out
 // Results are staged over the tile that has no reader left: dq over V, dk over Q, dv over K.  The tiles and states fill the SM's
-// shared memory, so that a CTA's loads overlap nothing but the set-up; the CTA after it finds its tiles in L2.
+// shared memory, so that a CTA's loads overlap nothing of the CTA before it: the scores begin when dO and V are there, the states and
+// the other tiles arrive meanwhile (172 -> 163 us at B1 H16 N16384 bf16, whose traffic alone takes 93), and the CTA after it finds
+// its tiles in L2 (3 us).
 // With k.dk split into what the chunk itself contributes and what lies across its end,
 //     dg_t = sum_{u>=t} (q_u.dq_u - (k_u.dk_u)_within) + sum_{s<t} (k_s.dk_s)_across + A <S, R>
 // counts the pairs that cross t and no others, but for those within the chunk, which are the same rounded products in q.dq and in
@@ -1107,15 +1109,16 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
 // and has its half of the accumulator beside it, so that a warp reads what it alone has written over; everything a group does per
 // chunk is a handful of rolled loops that all three run (the one-chunk kernel spent a quarter of its time waiting for instructions
 // and another at its barriers):
-//     scores, state's part (MMA) -> decay, pack -> rows (MMA) -> rows + scaled state's part -> result over a tile -> TMA
+//     scores, state's part (MMA) -> decay, pack -> rows (MMA) -> rows + scaled state's part -> the group's result tile -> TMA
 // dv has no room in TMEM for a second accumulator: its state's part goes where its rows will be added, and is scaled there first.
 //   warps 0-7: dq over Q     8-15: dk over K     16-23: dv over V     (rows and TMEM lanes 32 (w % 4) .., half (w / 4) % 2)
 //   warps 24-27: gates of the next chunk, masked rows, <S, R>, dg     warp 28: TMA loads
 //   warps 29-31, one thread each: the MMAs and the stores of a pass, so that the scores of the next chunk are under way while the
 //   last rows of this one are written, and no working warp spends its time on issuing
 // Two stages of (dO, V, K, Q, S, R), 80 KB, and a tile per group for its results, so that a stage is free as soon as the last group
-// has its products (staged over the tiles instead, a stage was held until the stores had been read, 2000 cycles of a chunk's
-// 8000); 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
+// has its products (staged over the tiles instead, a stage was held until the stores had been read: 2000 of a chunk's 8000 cycles).
+// B8 H16 N4096 bf16: 137 us, 3.6 TB/s; its traffic, states included, would take 83.  The schedulers issue in 64 % of the cycles:
+// what is left is instructions of the decays and of the rows.  L2 prefetches of the chunk after the next cost 8 us.  128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
 // state's part of dq and dk.
 // Barriers that a stage's chunk completes once are kept per stage, so that nobody can be a whole phase ahead of one that waits.
 // Every wait is bounded.  After one that gave up every further wait returns at once; the warps that share a named barrier go through
