@@ -1117,8 +1117,11 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
 //   last rows of this one are written, and no working warp spends its time on issuing
 // Two stages of (dO, V, K, Q, S, R), 80 KB, and a tile per group for its results, so that a stage is free as soon as the last group
 // has its products (staged over the tiles instead, a stage was held until the stores had been read: 2000 of a chunk's 8000 cycles).
-// B8 H16 N4096 bf16: 137 us, 3.6 TB/s; its traffic, states included, would take 83.  The schedulers issue in 64 % of the cycles:
-// what is left is instructions of the decays and of the rows.  L2 prefetches of the chunk after the next cost 8 us.  128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
+// B8 H16 N4096 bf16: 137 us, 3.6 TB/s; its traffic, states included, would take 83.  No single part bounds it (of 139 in one run:
+// 129 without the decays, 136 without the dot products, 135 without writing dg); the schedulers issue in 64 % of the cycles, and each group
+// waits for its own MMAs.  (One accumulator of 64 columns per group, half as many MMAs, is no faster: 136, and 1 % more for a
+// forward and a backward in turn.  L2 prefetches of the chunk after the next cost 8.)
+// 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
 // state's part of dq and dk.
 // Barriers that a stage's chunk completes once are kept per stage, so that nobody can be a whole phase ahead of one that waits.
 // Every wait is bounded.  After one that gave up every further wait returns at once; the warps that share a named barrier go through
