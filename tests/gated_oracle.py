@@ -1,5 +1,5 @@
 """Plain fp64 implementations of the gated scan and of the q/k norm with rotation, on the CPU, token by token; their gradients by
-autograd.  Checker only."""
+autograd.  For the tests only."""
 import torch
 
 
