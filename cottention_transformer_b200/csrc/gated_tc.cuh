@@ -565,15 +565,20 @@ __device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_l
     }
   }
 }
+// A state that is dropped is dropped whatever it holds: its products are left out, not multiplied by zero.
+template <int N>
+__device__ __forceinline__ void drop_if(bool dropped, uint32_t (&x)[N]) {
+  if (dropped) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = 0u;
+  }
+}
 // 32 columns of an accumulator, scaled by f (0: whatever they hold)
 __device__ __forceinline__ void acc_scaled(float (&acc)[32], uint32_t taddr_lane, float f) {
   uint32_t r[32];
   ptx::tmem_ld_x32(taddr_lane, r);
   ptx::tmem_ld_wait();
-  if (f == 0.f) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = 0u;
-  }
+  drop_if(f == 0.f, r);
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
     const float2 x = mul2(pair(r + j), make_float2(f, f));
@@ -1491,6 +1496,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
           uint32_t r[32];
           tmem_ld_x32(tMine + 32, r);
           tmem_ld_wait();
+          drop_if(scale == 0.f, r);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 x = mul2(pair(r + j), make_float2(scale, scale));
@@ -1529,6 +1535,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
           tmem_ld_wait();
           if (pass == 1) dot16_2<T>(dot, x, u, w);
           if (with_state) {
+            drop_if(scale == 0.f, y);
             if (pass == 1) dot16_2<T>(across, y, u, w);
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {

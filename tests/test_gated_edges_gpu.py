@@ -1,0 +1,53 @@
+"""The gated scan and its neighbours where a state, a mask or a gate is at its limit: against fp64, or against the same call without
+what must not matter."""
+import pytest
+import torch
+
+from test_gated_scan_gpu import _compare, _inputs, _truth
+
+pytestmark = pytest.mark.gpu
+
+
+def _call(q, k, v, g, keep, st, do, dst):
+    """Outputs and all gradients, the gates' and the initial state's among them."""
+    from cottention_transformer_b200 import gated_scan
+    leaf = [t.cuda().requires_grad_() for t in (q, k, v, g)] + ([] if st is None else [st.cuda().requires_grad_()])
+    out, final = gated_scan(*leaf[:4], keep=None if keep is None else keep.cuda(), initial_state=leaf[4] if st is not None else None, return_state=True)
+    outs, grads = ((out,), (do.cuda(),)) if dst is None else ((out, final), (do.cuda(), dst.cuda()))
+    return out, final, *torch.autograd.grad(outs, leaf, grads)
+
+
+HELD = [float("inf"), float("nan"), 1e5]  # (1e5: its copy in fp16 is an infinity)
+AT = [0, 5, 63, 130]  # the first position of the new document, at a border and inside a chunk
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("at", AT)
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_behind_a_dropped_state(dtype, D, at, held):
+    """Behind a gate of -inf outputs and gradients are those of a sequence that begins there, whatever the state before it holds."""
+    q, k, v, g, _, st, do, dst = _inputs(1, 2, 200, D, dtype, seed=40, init=True)
+    g[:, :, at] = float("-inf")
+    behind = slice(at, None)
+    got = _call(q, k, v, g, None, torch.full_like(st, held), do, dst)
+    want = _truth(*(t[:, :, behind] for t in (q, k, v, g)), None, None, do[:, :, behind], dst)
+    _compare([t[:, :, behind] if i != 1 else t for i, t in enumerate(got[:6])], want, dtype)
+
+
+def _before_a_drop(dtype, D, at, held):
+    """Before a gate of -inf the gradients are those of a sequence that ends there, whatever the gradient of the last state holds."""
+    q, k, v, g, _, st, do, dst = _inputs(1, 2, 200, D, dtype, seed=41, init=True)
+    g[:, :, at] = float("-inf")
+    before = slice(0, at)
+    got = _call(q, k, v, g, None, st, do, torch.full_like(dst, held))
+    want = _truth(*(t[:, :, before] for t in (q, k, v, g)), None, st, do[:, :, before], None)
+    _compare([got[0][:, :, before], want[1], *(t[:, :, before] for t in got[2:6]), got[6]], want, dtype)
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("at", AT[1:])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_before_a_dropped_state_gradient(dtype, D, at, held):
+    _before_a_drop(dtype, D, at, held)
