@@ -737,7 +737,7 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   if (with_state) {
     wait_bar_warp(&bar_mma[1], 0, abort_flag, kWaitChunkMma, chunk);
     tc_fence_after_sync();
-    acc_scaled(acc, tAcc + lane_base + 32 * hf, ex2(Gr));
+    acc_scaled(acc, tAcc + lane_base + 32 * hf, kp ? ex2(Gr) : 0.f);  // (a masked row is zero, whatever the state holds)
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) acc[j] = 0.f;
@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     if (with_R) times_state_t(tY, dV, sR, &bar_state[1]);
   });
   const float Gr = sG[row], total = sG[kGtChunk - 1];
-  const float head = ex2(Gr), tail = ex2(total - Gr);
+  const float head = kp ? ex2(Gr) : 0.f, tail = kp ? ex2(total - Gr) : 0.f;  // (a masked row is zero, whatever the states hold)
   const float row_low = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = ex2(sG[32 * wq + 31] - Gr);
   const int panel = cg / 2 * kTileBytes, j0 = 4 * (cg & 1);  // where this thread's 32 columns are in a row of D
 
@@ -1138,6 +1138,7 @@ constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage + 3 * kTileBytes;
 struct __align__(16) BwdInfo {  // of a chunk: one more than there are stages, so that a chunk's is made before its tiles arrive
   float G[kGtChunk], gate[kGtChunk];
   float low[192], up[192];  // column factors of row blocks 1, 2, 3 (32, 64, 96 columns) and 0, 1, 2 (96, 64, 32 columns)
+  uint32_t kept[4];         // unmasked rows, a bit each
   int has_s, has_r;
 };
 struct BwdDots {  // a stage's dot products, by halves of the columns
@@ -1325,6 +1326,8 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       gate_sums<false>(g, lane);
       if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
       f.gate[t] = gate_of<T>(own, a.gate_f32);
+      const uint32_t kept_rows = __ballot_sync(0xffffffffu, own.take != 0);
+      if (lane == 0) f.kept[wq] = kept_rows;
       if (t == 0) f.has_s = has_s(chunk), f.has_r = has_r(chunk);
       named_sync(4, 128);
 #pragma unroll
@@ -1488,7 +1491,8 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       tmem_st_wait();
       tc_fence_before_sync();
       warp_arrive(&bar_packed[pass], lane);
-      const float scale = ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr);
+      // (a masked row is zero, whatever the state holds)
+      const float scale = f.kept[wq] >> lane & 1u ? ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr) : 0.f;
       if (pass == 2) {
         if (with_state) {  // dv: the state's part, scaled where it is
           if (!wait(n, &bar_state[s])) break;

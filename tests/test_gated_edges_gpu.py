@@ -51,3 +51,26 @@ def _before_a_drop(dtype, D, at, held):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_gradients_before_a_dropped_state_gradient(dtype, D, at, held):
     _before_a_drop(dtype, D, at, held)
+
+
+@pytest.mark.parametrize("N", [20, 200])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_masked_rows_beside_states_that_are_not_finite(dtype, D, N):
+    """Padding in front of a document (its gate drops an initial state that holds an infinity) and at the end of a sequence whose
+    last state has an infinite gradient: outputs and gradients of masked rows are zero, those of the document what they are alone."""
+    q, k, v, g, _, st, do, dst = _inputs(2, 2, N, D, dtype, seed=42, init=True)
+    a, b = N // 4, N - N // 4
+    keep = torch.zeros(2, N, dtype=torch.bool)
+    keep[:, a:b] = True
+    g[:, :, a] = float("-inf")
+    got = _call(q, k, v, g, keep, torch.full_like(st, float("inf")), do, None)
+    doc = slice(a, b)
+    want = _truth(*(t[:, :, doc] for t in (q, k, v, g)), None, None, do[:, :, doc], None)
+    masked = ~keep[0].cuda()
+    for t in (got[0], *got[2:6]):
+        assert (t[:, :, masked] == 0).all()
+    _compare([t[:, :, doc] if i != 1 else t for i, t in enumerate(got[:6])], want, dtype)
+    got = _call(q, k, v, g, keep, st, do, torch.full_like(dst, float("inf")))
+    for t in (got[0], *got[2:6]):
+        assert (t[:, :, masked] == 0).all()
