@@ -1493,6 +1493,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       warp_arrive(&bar_packed[pass], lane);
       // (a masked row is zero, whatever the state holds)
       const float scale = f.kept[wq] >> lane & 1u ? ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr) : 0.f;
+      const bool dropped = __any_sync(0xffffffffu, scale == 0.f);
       if (pass == 2) {
         if (with_state) {  // dv: the state's part, scaled where it is
           if (!wait(n, &bar_state[s])) break;
@@ -1500,7 +1501,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
           uint32_t r[32];
           tmem_ld_x32(tMine + 32, r);
           tmem_ld_wait();
-          drop_if(scale == 0.f, r);
+          if (dropped) drop_if(scale == 0.f, r);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 x = mul2(pair(r + j), make_float2(scale, scale));
@@ -1539,7 +1540,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
           tmem_ld_wait();
           if (pass == 1) dot16_2<T>(dot, x, u, w);
           if (with_state) {
-            drop_if(scale == 0.f, y);
+            if (dropped) drop_if(scale == 0.f, y);
             if (pass == 1) dot16_2<T>(across, y, u, w);
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
