@@ -25,7 +25,9 @@ constexpr int kGtChunk = 128;
 constexpr int kStateTile = 64 * 128;      // bytes of a [64 x 64] 16-bit tile
 constexpr int kWalkThreads = 448;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kGateFloorTc = -200.f * kLog2e;  // e^-200 = 0 in fp32; sums of it keep their digits
+// In units of log 2: a gate down here drops the state (ex2 is zero below the smallest normal number, 2^-126).  In the walk, whose sums are
+// additions towards one end of a chunk only, it counts as this; the chunk kernels keep it out of their sums (DropBits).
+constexpr float kGateFloorTc = -128.f;
 
 enum { kWaitWalkTma = 16, kWaitWalkFree = 17, kWaitWalkPrep = 18, kWaitWalkState = 19, kWaitChunkTma = 20, kWaitChunkMma = 21 };
 
@@ -480,6 +482,38 @@ __global__ void __launch_bounds__(128) gated_patch_kernel(const GatedTcArgs a) {
   }
 }
 
+// The positions of a chunk whose gates drop the state, a bit each.  The chunk kernels take decays as differences of sums of gates: a
+// dropped state in such a sum would cost every later difference its digits, so the sums pass over these gates, and a decay across one
+// of them is zero by its bit.  Relative errors of the decays between neighbours of a document, worst and rms over 2000 chunks of gates
+// between 0 and -0.5 (these sums emulated on a CPU; float16 rounds by up to 4.9e-4): a quarter of the gates -inf, as a -288 in the
+// sums, 1.7e-3 and 1.7e-4, as a bit 6.6e-6 and 8e-7; every second gate -30, which is no drop, 4.2e-4 and 5e-5.
+struct __align__(16) DropBits {
+  uint32_t w[4];
+  // whether one of the positions first .. last does
+  __device__ __forceinline__ bool in(int first, int last) const {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = first - 32 * i, b = last - 32 * i;
+      const uint32_t from = a <= 0 ? 0xffffffffu : a > 31 ? 0u : 0xffffffffu << a, to = b >= 31 ? 0xffffffffu : b < 0 ? 0u : (2u << b) - 1u;
+      found |= w[i] & from & to;
+    }
+    return found;
+  }
+};
+// Of the 32 columns of a row's own block those that the row sees: LOWER: from the last drop up to the row, or the block's start, to the row;
+// else from the row to the position before the next drop, or the block's end.
+template <bool LOWER>
+__device__ __forceinline__ uint32_t seen_bits(uint32_t drops, int lane) {
+  if constexpr (LOWER) {
+    const uint32_t upto = (2u << lane) - 1u, d = drops & upto;
+    return d ? upto & (0xffffffffu << (31 - __clz(d))) : upto;
+  } else {
+    const uint32_t after = drops & ~((2u << lane) - 1u);
+    return (after ? (after & (0u - after)) - 1u : 0xffffffffu) & (0xffffffffu << lane);
+  }
+}
+
 struct GatedChunkArgs {
   const void* gate;
   const unsigned char* keep;
@@ -490,19 +524,55 @@ struct GatedChunkArgs {
   int H, N, nchunks, gate_f32, with_first, with_last;  // a state before the first chunk, a gradient after the last one
 };
 
+// A chunk's gates, four consecutive ones a lane: those that drop the state become 0 and a bit of `drops`, which is set only where there
+// are any.  Returns whether there are, for the whole warp.
+// (Functions of their own, this and drop_tables: what few chunks need is kept out of the loops.  Inline they cost the backward at head
+// dim 64 another 2 us of 172 at B8 H16 N4096.)
+__device__ __noinline__ float4 drops_taken(float4 x, DropBits* drops, int lane) {
+  float g[4] = {x.x, x.y, x.z, x.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (g[e] <= kGateFloorTc) g[e] = 0.f, bits |= 1u << (4 * (lane & 7) + e);
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, off);
+  if ((lane & 7) == 0) drops->w[lane >> 3] = bits;
+  return make_float4(g[0], g[1], g[2], g[3]);
+}
+__device__ __forceinline__ bool take_drops(float (&g)[4], DropBits& drops, int lane) {
+  const bool any = __any_sync(0xffffffffu, fminf(fminf(g[0], g[1]), fminf(g[2], g[3])) <= kGateFloorTc);
+  if (any) {
+    const float4 x = drops_taken(make_float4(g[0], g[1], g[2], g[3]), &drops, lane);
+    g[0] = x.x, g[1] = x.y, g[2] = x.z, g[3] = x.w;
+  }
+  return any;
+}
 // What the CTAs of both chunk kernels begin with: sums of the gates, and the column factors of the decays of the blocks off the
 // diagonal (LOWER: below it).
 template <typename T>
-__device__ __forceinline__ void chunk_gates(const GatedChunkArgs& a, float* sG, long b, int h, int c0, int lane) {
+__device__ __forceinline__ void chunk_gates(const GatedChunkArgs& a, float* sG, DropBits* drops, int* dropping, long b, int h, int c0, int lane) {
   float g[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) g[e] = gate_tc<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
+  const bool any = take_drops(g, *drops, lane);
+  if (lane == 0) *dropping = any;
   gate_sums<false>(g, lane);
   *reinterpret_cast<float4*>(&sG[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
 }
 template <bool LOWER>
-__device__ __forceinline__ void col_factor(float (*sCol)[kGtChunk], const float* sG, int w, int s) {
-  if (LOWER ? s < 32 * w : s >= 32 * w + 32) sCol[w][s] = ex2(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
+__device__ __forceinline__ void col_factor(float (*sCol)[kGtChunk], const float* sG, const DropBits& drops, bool dropping, int w, int s) {
+  if (LOWER ? s >= 32 * w : s < 32 * w + 32) return;
+  float f = ex2(LOWER ? sG[32 * w - 1] - sG[s] : sG[s] - sG[32 * w + 31]);
+  if (dropping && (LOWER ? drops.in(s + 1, 32 * w - 1) : drops.in(32 * w + 32, s))) f = 0.f;
+  sCol[w][s] = f;
+}
+// What drops change for a row (where there are any; few chunks have them): the columns of its own block that it sees, its factor for the
+// blocks off the diagonal.
+template <bool LOWER>
+__device__ __forceinline__ void row_drops(const DropBits& drops, int wq, int lane, uint32_t& seen, float& block) {
+  const uint32_t here = (2u << lane) - 1u, d = drops.w[wq];
+  seen = seen_bits<LOWER>(d, lane);
+  if (d & (LOWER ? here : ~here)) block = 0.f;
 }
 // Two products, two multiply-adds in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -527,9 +597,9 @@ __device__ __forceinline__ void dot16_2(float2& acc, const uint32_t* x, const ui
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc = fma2(Pack2<T>::unpack(p[j]), pair(x + 2 * j), acc);
 }
-// 32 columns (block `blk`) of the scores of a row of block wq, decayed, masked and packed
+// 32 columns (block `blk`) of the scores of a row of block wq, decayed, masked (`seen`: in the row's own block) and packed
 template <typename T, bool LOWER>
-__device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_lane, int blk, int wq, int lane, float Gr, float rowf, const float* sG,
+__device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_lane, int blk, int wq, uint32_t seen, float Gr, float rowf, const float* sG,
                                             const float* col) {
   if (LOWER ? blk > wq : blk < wq) {
 #pragma unroll
@@ -540,7 +610,6 @@ __device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_l
   ptx::tmem_ld_x32(taddr_lane + 32 * blk, r);
   ptx::tmem_ld_wait();
   if (blk == wq) {
-    const uint32_t keep_bits = LOWER ? (2u << lane) - 1u : 0xffffffffu << lane;
     const float sign = LOWER ? 1.f : -1.f;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
@@ -549,8 +618,8 @@ __device__ __forceinline__ void decay_block(uint32_t (&pk)[16], uint32_t taddr_l
       for (int e = 0; e < 4; e += 2) {
         float2 x = fma2(make_float2(-sign, -sign), e ? make_float2(Gs.z, Gs.w) : make_float2(Gs.x, Gs.y), make_float2(sign * Gr, sign * Gr));
         x = mul2(make_float2(ex2(x.x), ex2(x.y)), pair(r + j + e));
-        x.x = keep_bits & (1u << (j + e)) ? x.x : 0.f;
-        x.y = keep_bits & (2u << (j + e)) ? x.y : 0.f;
+        x.x = seen & (1u << (j + e)) ? x.x : 0.f;
+        x.y = seen & (2u << (j + e)) ? x.y : 0.f;
         pk[(j + e) / 2] = Pack2<T>::pack(x.x, x.y);
       }
     }
@@ -639,6 +708,8 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
   __shared__ __align__(16) float sG[kGtChunk], sCol[4][kGtChunk];  // (read four at a time)
+  __shared__ DropBits drops;  // (where `dropping`)
+  __shared__ int dropping;
   volatile int* abort_flag = &abort_flag_s;
 
   const int tid = threadIdx.x, lane = tid & 31;
@@ -682,12 +753,12 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
     }
     __syncwarp();
   } else if (warp == 4) {
-    chunk_gates<T>(a, sG, b, h, c0, lane);
+    chunk_gates<T>(a, sG, &drops, &dropping, b, h, c0, lane);
   }
   const bool kp = !a.keep || (c0 + row < a.N && a.keep[b * a.N + c0 + row]);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) col_factor<true>(sCol, sG, 2 * i + (tid >> 7), tid & 127);
+  for (int i = 0; i < 2; ++i) col_factor<true>(sCol, sG, drops, dropping, 2 * i + (tid >> 7), tid & 127);
   if (a.keep) {  // nothing of a masked position gets into a product
     wait_bar_warp(&bar_full, 0, abort_flag, kWaitChunkTma, chunk);
     if (!kp) {
@@ -713,10 +784,17 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   }
   wait_bar_warp(&bar_mma[0], 0, abort_flag, kWaitChunkMma, chunk);
   tc_fence_after_sync();
-  const float Gr = sG[row], rowf = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f);
+  const float Gr = sG[row];
+  float rowf = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f);
+  uint32_t seen = (2u << lane) - 1u;
+  bool with_row = kp;  // (a masked row is zero, whatever the state holds)
+  if (dropping) {
+    row_drops<true>(drops, wq, lane, seen, rowf);
+    with_row = kp && !drops.in(0, row);
+  }
   uint32_t pk[2][16];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) decay_block<T, true>(pk[i], tP + lane_base, 2 * hf + i, wq, lane, Gr, rowf, sG, sCol[wq]);
+  for (int i = 0; i < 2; ++i) decay_block<T, true>(pk[i], tP + lane_base, 2 * hf + i, wq, seen, Gr, rowf, sG, sCol[wq]);
   tc_fence_before_sync();
   __syncthreads();  // all scores have been read: their columns become P (the first 64) and the accumulator
   if (with_state && warp == 0) {
@@ -737,7 +815,7 @@ gated_fwd_tc_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_const
   if (with_state) {
     wait_bar_warp(&bar_mma[1], 0, abort_flag, kWaitChunkMma, chunk);
     tc_fence_after_sync();
-    acc_scaled(acc, tAcc + lane_base + 32 * hf, kp ? ex2(Gr) : 0.f);  // (a masked row is zero, whatever the state holds)
+    acc_scaled(acc, tAcc + lane_base + 32 * hf, with_row ? ex2(Gr) : 0.f);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) acc[j] = 0.f;
@@ -816,6 +894,8 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag_s;
   __shared__ __align__(16) float sG[kGtChunk], sLow[4][kGtChunk], sUp[4][kGtChunk];
+  __shared__ DropBits drops;  // (where `dropping`)
+  __shared__ int dropping;
   __shared__ float sQd[NG][kGtChunk], sKd[NG][kGtChunk], sBd[NG][kGtChunk], sCross[4 * NG], sPart[8];
   volatile int* abort_flag = &abort_flag_s;
 
@@ -881,13 +961,13 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     }
     __syncwarp();
   } else if (warp == 4) {
-    chunk_gates<T>(a, sG, b, h, c0, lane);
+    chunk_gates<T>(a, sG, &drops, &dropping, b, h, c0, lane);
   }
   const bool kp = !a.keep || (c0 + row < a.N && a.keep[b * a.N + c0 + row]);
   __syncthreads();
   for (int e = tid; e < 4 * kGtChunk; e += kBwd128Threads) {
-    col_factor<true>(sLow, sG, e >> 7, e & 127);
-    col_factor<false>(sUp, sG, e >> 7, e & 127);
+    col_factor<true>(sLow, sG, drops, dropping, e >> 7, e & 127);
+    col_factor<false>(sUp, sG, drops, dropping, e >> 7, e & 127);
   }
   // (every thread reads rows of the tiles later on, so every thread waits for them; nothing of a masked position gets into a product)
   auto arrived = [&](int which, unsigned char* tiles) {
@@ -963,8 +1043,15 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     if (with_R) times_state_t(tY, dV, sR, &bar_state[1]);
   });
   const float Gr = sG[row], total = sG[kGtChunk - 1];
-  const float head = kp ? ex2(Gr) : 0.f, tail = kp ? ex2(total - Gr) : 0.f;  // (a masked row is zero, whatever the states hold)
-  const float row_low = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = ex2(sG[32 * wq + 31] - Gr);
+  float head = kp ? ex2(Gr) : 0.f, tail = kp ? ex2(total - Gr) : 0.f;  // (a masked row is zero, whatever the states hold)
+  float row_low = ex2(wq > 0 ? Gr - sG[32 * wq - 1] : 0.f), row_up = ex2(sG[32 * wq + 31] - Gr);
+  uint32_t seen_low = (2u << lane) - 1u, seen_up = 0xffffffffu << lane;
+  if (dropping) {
+    row_drops<true>(drops, wq, lane, seen_low, row_low);
+    row_drops<false>(drops, wq, lane, seen_up, row_up);
+    if (drops.in(0, row)) head = 0.f;
+    if (drops.in(row + 1, kGtChunk - 1)) tail = 0.f;
+  }
   const int panel = cg / 2 * kTileBytes, j0 = 4 * (cg & 1);  // where this thread's 32 columns are in a row of D
 
   uint32_t pk[16];
@@ -973,7 +1060,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   for (int j = 0; j < 32; ++j) ax[j] = 0.f, ay[j] = 0.f;
   // ---- dq: decayed scores X (packed over what the other warps of the rows have read), the state's part
   wait(&bar_score[0]);
-  decay_block<T, true>(pk, tX + my_scores, cg, wq, lane, Gr, row_low, sG, sLow[wq]);
+  decay_block<T, true>(pk, tX + my_scores, cg, wq, seen_low, Gr, row_low, sG, sLow[wq]);
   sync();
   put_scores(tX, pk);
   if (with_S) {
@@ -982,7 +1069,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   }
   // ---- dk: the same in Y
   wait(&bar_score[1]);
-  decay_block<T, false>(pk, tY + my_scores, cg, wq, lane, Gr, row_up, sG, sUp[wq]);
+  decay_block<T, false>(pk, tY + my_scores, cg, wq, seen_up, Gr, row_up, sG, sUp[wq]);
   arrived(2, sQ);
   sync();
   issue(true, [&] { times_rows(tX, sK, &bar_rows[0]); });
@@ -1029,7 +1116,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
   });
   // ---- dv: decayed scores X
   wait(&bar_score[2]);
-  decay_block<T, false>(pk, tX + my_scores, cg, wq, lane, Gr, row_up, sG, sUp[wq]);
+  decay_block<T, false>(pk, tX + my_scores, cg, wq, seen_up, Gr, row_up, sG, sUp[wq]);
   sync();
   put_scores(tX, pk);
   // ---- dk out
@@ -1095,7 +1182,7 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
     float sr = 0.f;
 #pragma unroll
     for (int i = 0; i < 4 * NG; ++i) sr += sCross[i];
-    const float A = ex2(total);
+    const float A = dropping ? 0.f : ex2(total);
     x += A == 0.f ? 0.f : A * sr;
     for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
     const int pos = c0 + row;
@@ -1136,17 +1223,29 @@ constexpr int kBwd64Stage = 4 * kTileBytes + 2 * kStateTile;
 constexpr size_t kBwd64Smem = 1024 + 2 * kBwd64Stage + 3 * kTileBytes;
 
 struct __align__(16) BwdInfo {  // of a chunk: one more than there are stages, so that a chunk's is made before its tiles arrive
-  float G[kGtChunk], gate[kGtChunk];
+  float G[kGtChunk];
   float low[192], up[192];  // column factors of row blocks 1, 2, 3 (32, 64, 96 columns) and 0, 1, 2 (96, 64, 32 columns)
-  uint32_t kept[4];         // unmasked rows, a bit each
-  int has_s, has_r;
-};
-struct BwdDots {  // a stage's dot products, by halves of the columns
-  float qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];
+  DropBits drops;                 // (where `dropping`)
+  uint32_t from_s[4], from_r[4];  // unmasked rows that no drop parts from the state before, after the chunk: a bit each
+  int has_s, has_r, dropping;
 };
 __device__ __forceinline__ int low_at(int w) { return 16 * w * (w - 1); }                      // of column 0 of row block w
 __device__ __forceinline__ int up_at(int w) { return (w == 0 ? 0 : w == 1 ? 96 : 160) - 32 * (w + 1); }
-
+// What the drops of a chunk change in its tables.  Thread t of four warps, `rows`: the unmasked rows of the warp.
+__device__ __noinline__ void drop_tables(BwdInfo* f, int t, uint32_t rows) {
+  const DropBits drops = f->drops;
+#pragma unroll 1
+  for (int w = 0; w < 3; ++w) {
+    if (t < 32 * w + 32 && drops.in(t + 1, 32 * w + 31)) f->low[low_at(w + 1) + t] = 0.f;
+    if (t >= 32 * w + 32 && drops.in(32 * w + 32, t)) f->up[up_at(w) + t] = 0.f;
+  }
+  const uint32_t rows_s = rows & __ballot_sync(0xffffffffu, !drops.in(0, t)), rows_r = rows & __ballot_sync(0xffffffffu, !drops.in(t + 1, kGtChunk - 1));
+  __syncwarp();
+  if ((t & 31) == 0) f->from_s[t >> 5] = rows_s, f->from_r[t >> 5] = rows_r;
+}
+struct BwdDots {  // a stage's dot products, by halves of the columns
+  float qd[2][kGtChunk], kd[2][kGtChunk], bd[2][kGtChunk];
+};
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 template <typename T>
@@ -1306,7 +1405,8 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
   } else if (warp >= 24) {
     // ---------------------------------------------------------------- gates, masked rows, <S, R>, dg
     const int t = tid - 768;  // position
-    RawGate raw[4], own = {0u, 1};
+    RawGate raw[4];
+    bool own_take = true;  // whether row t counts
     float cross_before = 0.f;
     bool kp_before = true;
     auto fetch = [&](long unit) {
@@ -1314,7 +1414,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       const int c0 = static_cast<int>(unit % a.nchunks) * kGtChunk, h = static_cast<int>(bh % a.H);
 #pragma unroll
       for (int e = 0; e < 4; ++e) raw[e] = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + 4 * lane + e);
-      own = gate_raw<T>(a.gate, a.keep, a.sg, a.gate_f32, a.N, b, h, c0 + t);
+      if (a.keep) own_take = c0 + t < a.N && a.keep[b * a.N + c0 + t];
     };
     // the sums of a chunk's gates and the column factors, from what was fetched
     auto make_tables = [&](int n, int chunk) {
@@ -1323,18 +1423,19 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       float g[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) g[e] = gate_of<T>(raw[e], a.gate_f32);
+      const bool dropping = take_drops(g, f.drops, lane);  // (the four warps write the same)
       gate_sums<false>(g, lane);
       if (wq == 0) *reinterpret_cast<float4*>(&f.G[4 * lane]) = make_float4(g[0], g[1], g[2], g[3]);
-      f.gate[t] = gate_of<T>(own, a.gate_f32);
-      const uint32_t kept_rows = __ballot_sync(0xffffffffu, own.take != 0);
-      if (lane == 0) f.kept[wq] = kept_rows;
-      if (t == 0) f.has_s = has_s(chunk), f.has_r = has_r(chunk);
+      if (t == 0) f.has_s = has_s(chunk), f.has_r = has_r(chunk), f.dropping = dropping;
       named_sync(4, 128);
 #pragma unroll
       for (int w = 0; w < 3; ++w) {
         if (t < 32 * w + 32) f.low[low_at(w + 1) + t] = ex2(f.G[32 * w + 31] - f.G[t]);
         if (t >= 32 * w + 32) f.up[up_at(w) + t] = ex2(f.G[t] - f.G[32 * w + 31]);
       }
+      const uint32_t rows = __ballot_sync(0xffffffffu, own_take);
+      if (lane == 0) f.from_s[wq] = rows, f.from_r[wq] = rows;
+      if (dropping) drop_tables(&f, t, rows);
     };
     // dg of a chunk that is done (unit u, the n-th of this CTA): its dot products, <S, R> as this warp's part
     auto write_dgate = [&](long u, int n, float cross, bool kept) {
@@ -1355,11 +1456,11 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       if (lane == 31) sPart[4 + wq] = up;
       const float before = __shfl_up_sync(0xffffffffu, up, 1);
       named_sync(4, 128);
-      const float A = ex2(f.G[kGtChunk - 1]);
+      const float A = f.dropping ? 0.f : ex2(f.G[kGtChunk - 1]);
       float x = run + (lane ? before : 0.f) + (A == 0.f ? 0.f : A * ((sPart[8] + sPart[9]) + (sPart[10] + sPart[11])));
       for (int w = 0; w < 4; ++w) x += w > wq ? sPart[w] : w < wq ? sPart[4 + w] : 0.f;
       if (pos < a.N && !*abort_flag) {
-        if (!kept || (pos == 0 && !a.with_first) || f.gate[t] <= kGateFloorTc) x = 0.f;
+        if (!kept || (pos == 0 && !a.with_first) || (f.dropping && f.drops.w[wq] >> lane & 1u)) x = 0.f;
         const long long o = b * a.sdg.b + h * a.sdg.h + static_cast<long long>(pos) * a.sdg.n;
         if (a.gate_f32)
           static_cast<float*>(a.dgate)[o] = x;
@@ -1373,7 +1474,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     if (unit < a.units) {
       fetch(unit);
       make_tables(0, static_cast<int>(unit % a.nchunks));
-      kept = own.take != 0;
+      kept = own_take;
       if (unit + gridDim.x < a.units) fetch(unit + gridDim.x);
     }
     for (; unit < a.units; unit += gridDim.x, ++n) {
@@ -1409,7 +1510,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       const bool kept_now = kept;
       if (unit + gridDim.x < a.units) {
         make_tables(n + 1, static_cast<int>((unit + gridDim.x) % a.nchunks));
-        kept = own.take != 0;
+        kept = own_take;
         if (unit + 2 * static_cast<long>(gridDim.x) < a.units) fetch(unit + 2 * static_cast<long>(gridDim.x));
       }
       if (n > 0) write_dgate(unit - gridDim.x, n - 1, cross_before, kp_before);
@@ -1424,7 +1525,6 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
     const uint32_t tMine = tmem + 128 * pass + 64 * half + lane_base;
     const float sign = lower ? 1.f : -1.f;
     const uint32_t tState = tmem + 384 + 64 * pass + 32 * half + lane_base;
-    const uint32_t keep_bits = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of a diagonal block's columns
     // several barriers at once: one round trip
     auto wait = [&](int n, auto... bars) {
       const uint32_t parity = (n >> 1) & 1;
@@ -1448,7 +1548,14 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       tc_fence_after_sync();
       const bool with_state = lower ? f.has_s : f.has_r;
       const float Gr = f.G[row], signedG = sign * Gr;
-      const float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
+      float rowf = ex2(lower ? (wq > 0 ? Gr - f.G[32 * wq - 1] : 0.f) : f.G[32 * wq + 31] - Gr);
+      uint32_t seen = lower ? (2u << lane) - 1u : 0xffffffffu << lane;  // of the diagonal block's columns
+      if (f.dropping) {
+        if (lower)
+          row_drops<true>(f.drops, wq, lane, seen, rowf);
+        else
+          row_drops<false>(f.drops, wq, lane, seen, rowf);
+      }
       const float* col = lower ? f.low + low_at(wq) : f.up + up_at(wq);  // (of a block without factors: not read)
       // decayed, masked, packed in place: the half's first 32 columns into its first 16, then the others into the next 16
 #pragma unroll 1
@@ -1470,8 +1577,8 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
               for (int e = 0; e < 4; e += 2) {
                 float2 x = fma2(make_float2(-sign, -sign), e ? make_float2(Gs.z, Gs.w) : make_float2(Gs.x, Gs.y), make_float2(signedG, signedG));
                 x = mul2(make_float2(ex2(x.x), ex2(x.y)), pair(r + j + e));
-                x.x = keep_bits & (1u << (j + e)) ? x.x : 0.f;
-                x.y = keep_bits & (2u << (j + e)) ? x.y : 0.f;
+                x.x = seen & (1u << (j + e)) ? x.x : 0.f;
+                x.y = seen & (2u << (j + e)) ? x.y : 0.f;
                 pk[(j + e) / 2] = Pack2<T>::pack(x.x, x.y);
               }
             }
@@ -1492,7 +1599,7 @@ __global__ void __launch_bounds__(kBwd64Threads, 1) gated_bwd64_kernel(const __g
       tc_fence_before_sync();
       warp_arrive(&bar_packed[pass], lane);
       // (a masked row is zero, whatever the state holds)
-      const float scale = f.kept[wq] >> lane & 1u ? ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr) : 0.f;
+      const float scale = (lower ? f.from_s[wq] : f.from_r[wq]) >> lane & 1u ? ex2(lower ? Gr : f.G[kGtChunk - 1] - Gr) : 0.f;
       const bool dropped = __any_sync(0xffffffffu, scale == 0.f);
       if (pass == 2) {
         if (with_state) {  // dv: the state's part, scaled where it is

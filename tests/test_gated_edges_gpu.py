@@ -74,3 +74,37 @@ def test_masked_rows_beside_states_that_are_not_finite(dtype, D, N):
     got = _call(q, k, v, g, keep, st, do, torch.full_like(dst, float("inf")))
     for t in (got[0], *got[2:6]):
         assert (t[:, :, masked] == 0).all()
+
+
+@pytest.mark.parametrize("gate", [float("-inf"), -1e4, -100.0])
+@pytest.mark.parametrize("roles", ["scores", "rows"])
+@pytest.mark.parametrize("N", [128, 300])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_decays_inside_documents_of_a_few_tokens(dtype, D, N, roles, gate):
+    """Packed documents of 2 to 8 tokens.  The inputs are such that every entry of a result is one decay: either all scores are 1 and the
+    rows are unit vectors of their position, or the other way round.  A decay is rounded to the type once (u); its exponent is a
+    difference of two sums of at most 128 gates below 0.5 / log 2, i.e. numbers below 128 (half an ulp: 2^-18) after at most eight
+    additions each: 16 x 2^-18 x log 2 = 4.3e-5, less than 0.1 u of float16.  No document begins within a chunk and ends in the next."""
+    r = torch.Generator().manual_seed(43)
+    g = -0.5 * torch.rand(1, 1, N, generator=r)
+    starts, t = [], 0
+    while t < N:
+        starts.append(t)
+        t = min(t + int(torch.randint(2, 9, (1,), generator=r)), (t // 128 + 1) * 128)
+    g[..., starts] = gate
+    first = torch.zeros(N, dtype=torch.long)
+    first[starts] = 1
+    doc = first.cumsum(0)
+    sums = torch.where(first.bool(), 0.0, g[0, 0].double()).cumsum(0)
+    pos = torch.arange(N)
+    W = (sums[:, None] - sums[None]).exp() * ((doc[:, None] == doc[None]) & (pos[:, None] >= pos[None]))  # [t, s]
+    unit = torch.eye(D, dtype=dtype)[pos % D].view(1, 1, N, D)
+    ones = torch.eye(D, dtype=dtype)[:1].expand(N, D).reshape(1, 1, N, D)
+    qk, vo = (ones, unit) if roles == "scores" else (unit, ones)
+    out, _, dq, dk, dv, _ = _call(qk, qk, vo, g, None, None, vo, None)
+    at = unit[0, 0].double()
+    # out_t and dq_t: entry s of row t is the decay from s to t; dv_s and dk_s: entry t of row s
+    for got, want in ((out, W @ at), (dv, W.T @ at)) if roles == "scores" else ((dq, W @ at), (dk, W.T @ at)):
+        got = got[0, 0].double().cpu()
+        assert ((got - want).abs() <= 1.1 * torch.finfo(dtype).eps / 2 * want).all(), ((got - want).abs() / want.clamp(min=1e-9)).max()
