@@ -394,8 +394,9 @@ __global__ void __launch_bounds__(kGsThreads, D > 64 ? 1 : 3) gated_chunk_kernel
   }
 }
 
-// dg of a chunk.  A dropped state (the gate at or below its floor) has no gradient, nor has the first gate of a sequence that starts
-// from nothing, nor a masked one.  grid = B*H * chunks.
+// dg of a chunk.  Nothing crosses a gate that drops the state (e^g = 0 in fp32): what lies behind it is left out of the sums before it,
+// whatever it holds.  Such a gate has no gradient, nor has the first gate of a sequence that starts from nothing, nor a masked one.
+// grid = B*H * chunks.
 template <typename T, int D>
 __global__ void __launch_bounds__(kGsThreads) gated_dgate_kernel(const GatedArgs g) {
   __shared__ double part[kGsThreads / 32];
@@ -423,21 +424,32 @@ __global__ void __launch_bounds__(kGsThreads) gated_dgate_kernel(const GatedArgs
     cross = 0.0;
 #pragma unroll
     for (int w = 0; w < kGsThreads / 32; ++w) cross += part[w];
-    // lane l has positions 63 - 2 l and 62 - 2 l: an inclusive sum from the chunk's end
+    // lane l has positions 63 - 2 l and 62 - 2 l.  The sum at a position is its own term and, unless the next gate drops the state,
+    // the sum there; the last position's next one is the chunk's end, whose sum is <S', R>.
+    const int p1 = c0 + 63 - 2 * lane;
     const double d1 = d[63 - 2 * lane], d0 = d[62 - 2 * lane];
-    double run = d1 + d0;
+    const bool drop1 = p1 < g.N && expf(static_cast<float>(gated_gate<T>(g, b, h, p1))) == 0.f,
+               drop0 = p1 - 1 < g.N && expf(static_cast<float>(gated_gate<T>(g, b, h, p1 - 1))) == 0.f;
+    double run = drop0 ? 0.0 : drop1 ? d0 : d0 + d1;  // of what the positions of lanes up to this one hand on, their own part
+    int open = !drop0 && !drop1;                      // whether they hand on what comes from behind them
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const double up = __shfl_up_sync(0xffffffffu, run, off);
-      if (lane >= off) run += up;
+      const int up_open = __shfl_up_sync(0xffffffffu, open, off);
+      if (lane >= off && open) run += up, open = up_open;
     }
-    const double sums[2] = {run - d0 + cross, run + cross};
+    double in = __shfl_up_sync(0xffffffffu, run, 1);
+    const int in_open = __shfl_up_sync(0xffffffffu, open, 1);
+    in = lane == 0 ? cross : in_open ? in + cross : in;
+    const double at1 = d1 + in, at0 = drop1 ? d0 : d0 + at1;
+    const double sums[2] = {at1, at0};
+    const bool drops[2] = {drop1, drop0};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int pos = c0 + 63 - 2 * lane - u;
       if (pos < g.N) {
         const bool masked = g.keep && !g.keep[b * g.N + pos];
-        const bool none = masked || (pos == 0 && !g.with_initial) || gated_gate<T>(g, b, h, pos) <= kGateFloor;
+        const bool none = masked || (pos == 0 && !g.with_initial) || drops[u];
         const float x = none ? 0.f : static_cast<float>(sums[u]);
         const long long o = gated_at(g.sdg, b, h, pos);
         if (g.gate_f32)

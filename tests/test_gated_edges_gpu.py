@@ -108,3 +108,10 @@ def test_decays_inside_documents_of_a_few_tokens(dtype, D, N, roles, gate):
     for got, want in ((out, W @ at), (dv, W.T @ at)) if roles == "scores" else ((dq, W @ at), (dk, W.T @ at)):
         got = got[0, 0].double().cpu()
         assert ((got - want).abs() <= 1.1 * torch.finfo(dtype).eps / 2 * want).all(), ((got - want).abs() / want.clamp(min=1e-9)).max()
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("at", AT[1:])
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 32), (torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 32), (torch.float16, 32)])
+def test_gradients_before_a_dropped_state_gradient_on_cuda_cores(dtype, D, at, held):
+    _before_a_drop(dtype, D, at, held)
