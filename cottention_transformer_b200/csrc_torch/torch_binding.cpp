@@ -616,6 +616,14 @@ GatedCall gated_fwd(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor
         "cott_gated_scan_fwd");
   return c;
 }
+// the same as an operator, for what records or chooses operators (no final state: an empty tensor)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_fwd_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                                                            const OptTensor& keep, const OptTensor& initial, bool return_state) {
+  check_gated("gated_scan", q, k, v, log_decay);
+  if (has(initial)) check_gated_state("initial_state", *initial, q);
+  GatedCall c = gated_fwd(q, k, v, log_decay, keep, initial, return_state);
+  return {c.out, return_state ? c.final : at::empty({0}, q.options().dtype(at::kFloat)), c.states};
+}
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& gate,
                                const OptTensor& keep, const OptTensor& initial, bool return_state, bool want_dinitial) {
@@ -751,8 +759,7 @@ struct QKNormFn : torch::autograd::Function<QKNormFn> {
     return {dq, dk, dqw, dkw, Variable(), Variable(), Variable()};
   }
 };
-variable_list qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const OptTensor& sin,
-                             const OptTensor& cos, double eps) {
+void check_norm(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw) {
   TORCH_CHECK(q.is_cuda() && k.is_cuda() && qw.is_cuda() && kw.is_cuda(), "qk_norm_rotary needs CUDA tensors (there is no CPU path)");
   if (q.dim() != 4 || k.dim() != 4)
     throw py::value_error("[B, H, N, D] tensors expected, got " + std::to_string(q.dim()) + " and " + std::to_string(k.dim()) + " dimensions");
@@ -767,11 +774,21 @@ variable_list qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at:
     TORCH_CHECK(w.sizes() == at::IntArrayRef({D}) && (w.scalar_type() == at::kFloat || w.scalar_type() == t) && w.scalar_type() == qw.scalar_type(),
                 "the weights must be [D] = [", D, "], both in float32 or both of the tensors' type, got ", w.sizes(), " in ", w.scalar_type());
   TORCH_CHECK(k.device() == q.device() && qw.device() == q.device() && kw.device() == q.device(), "q, k and the weights must be on one device");
+}
+variable_list qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const OptTensor& sin,
+                             const OptTensor& cos, double eps) {
+  check_norm(q, k, qw, kw);
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || qw.requires_grad() || kw.requires_grad())) {
     const NormCall c(q, k, qw, kw, sin, cos, eps);
     return {c.q_out, c.k_out};
   }
   return QKNormFn::apply(q, k, qw, kw, sin, cos, eps);
+}
+std::tuple<at::Tensor, at::Tensor> qk_norm_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const OptTensor& sin,
+                                               const OptTensor& cos, double eps) {
+  check_norm(q, k, qw, kw);
+  const NormCall c(q, k, qw, kw, sin, cos, eps);
+  return {c.q_out, c.k_out};
 }
 
 // what Python calls
@@ -800,6 +817,9 @@ TORCH_LIBRARY(cottention_b200, m) {
   m.def("causal_fwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, int nseg, bool save_states) -> (Tensor, Tensor, Tensor)");
   m.def("causal_bwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, Tensor dout, Tensor ws, Tensor saved, int nseg) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("bidir_fwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep) -> (Tensor, Tensor)");
+  m.def("gated_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? keep, Tensor? initial_state, bool return_state) -> (Tensor, Tensor, Tensor)");
+  m.def("gated_step(Tensor(a!) state, Tensor q, Tensor k, Tensor v, Tensor log_decay) -> Tensor");
+  m.def("qk_norm_fwd(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor? sin, Tensor? cos, float eps) -> (Tensor, Tensor)");
   m.def("gated_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? keep, bool with_initial, Tensor states, Tensor dout, Tensor? dfinal, bool want_dinitial) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("qk_norm_bwd(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor? sin, Tensor? cos, Tensor dq_out, Tensor dk_out, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("bidir_bwd(Tensor q, Tensor k, Tensor v, Tensor norm_const, Tensor? keep, Tensor dout, Tensor scratch) -> (Tensor, Tensor, Tensor, Tensor)");
@@ -809,6 +829,9 @@ TORCH_LIBRARY_IMPL(cottention_b200, CUDA, m) {
   m.impl("causal_bwd", &causal_bwd);
   m.impl("bidir_fwd", &bidir_fwd);
   m.impl("bidir_bwd", &bidir_bwd);
+  m.impl("gated_fwd", &gated_fwd_op);
+  m.impl("gated_step", &gated_step);
+  m.impl("qk_norm_fwd", &qk_norm_fwd);
   m.impl("gated_bwd", &gated_bwd);
   m.impl("qk_norm_bwd", &qk_norm_bwd);
 }

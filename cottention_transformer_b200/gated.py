@@ -87,6 +87,13 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx, q, k, v, log_decay, keep, initial_state, return_state):
         q, k, v, init = rows16(q), rows16(k), rows16(v), _state16(initial_state)
         kp = None if keep is None else keep.to(torch.uint8, memory_format=torch.contiguous_format, copy=True)
+        ctx.save_for_backward(q, k, v, log_decay)
+        ctx.kp, ctx.with_initial = kp, init is not None
+        ctx.set_materialize_grads(False)
+        ops = _binding.visible_ops()
+        if ops is not None:
+            out, final, ctx.states = ops.gated_fwd(q, k, v, log_decay, kp, init, return_state)
+            return (out, final) if return_state else out
         B, H, N, D = q.shape
         code, gcode = _lib.DTYPE_CODE[q.dtype], _lib.DTYPE_CODE[log_decay.dtype]
         L = _lib.lib()
@@ -99,9 +106,7 @@ class _GatedScan(torch.autograd.Function):
                                        _lib.ptr(final), _lib.ptr(states), _lib.ptr(ws), _layout(q, k, v, out, log_decay), B, H, N, D, code, gcode,
                                        _lib.stream_ptr(q.device))
         _lib.check(st, "cott_gated_scan_fwd")
-        ctx.save_for_backward(q, k, v, log_decay)
-        ctx.kp, ctx.states, ctx.with_initial = kp, states, init is not None
-        ctx.set_materialize_grads(False)
+        ctx.states = states
         return (out, final) if return_state else out
 
     @staticmethod
@@ -157,6 +162,10 @@ def gated_scan_step(state, q, k, v, log_decay):
     m = _binding.autograd()
     if m is not None:
         return m.gated_step(state, q, k, v, log_decay)
+    _binding.refuse_transforms("gated_scan_step", state, q, k, v, log_decay)
+    ops = _binding.visible_ops()
+    if ops is not None:
+        return ops.gated_step(state, q, k, v, log_decay)
     _check("gated_scan_step", q, k, v, log_decay)
     _check_state("state", state, q)
     if not state.is_contiguous() or state.data_ptr() % 16:

@@ -61,6 +61,11 @@ class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, sin, cos, eps):
         q, k, qw, kw = rows16(q), rows16(k), q_weight.contiguous(), k_weight.contiguous()
+        ctx.save_for_backward(q, k, qw, kw, sin, cos)
+        ctx.eps = eps
+        ops = _binding.visible_ops()
+        if ops is not None:
+            return ops.qk_norm_fwd(q, k, qw, kw, sin, cos, eps)
         B, Hq, N, D = q.shape
         q_out, k_out = torch.empty_like(q), torch.empty_like(k)
         with torch.cuda.device(q.device):
@@ -68,8 +73,6 @@ class _QKNormRotary(torch.autograd.Function):
                                              _lib.ptr(k_out), _layout(q, k, q_out, k_out), B, Hq, k.shape[1], N, D, eps, _lib.DTYPE_CODE[q.dtype],
                                              _lib.DTYPE_CODE[qw.dtype], _lib.stream_ptr(q.device))
         _lib.check(st, "cott_qk_norm_fwd")
-        ctx.save_for_backward(q, k, qw, kw, sin, cos)
-        ctx.eps = eps
         return q_out, k_out
 
     @staticmethod
