@@ -60,14 +60,14 @@ def visible_ops():
     return ops() if transformed() else None
 
 
-def refuse_transforms(what, *tensors):
+def refuse_transforms(what, *tensors, traced=True):
     """For calls that write a state in place and are no autograd functions: an error where a transform would drop its part of the
-    call (tangents, batched tensors) or a trace the call itself."""
+    call (tangents, batched tensors) or a trace the call itself.  traced: the call has an operator that a trace can record."""
     if _compiling():
         return
     if _functorch() is not None:
         raise RuntimeError(f"{what} writes its state in place: it cannot be transformed (vmap, grad, jvp, ...)")
     if _fw._current_level >= 0 and any(_fw.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} is not differentiable, in forward mode neither")
-    if _tracing() and ops() is None:
-        raise RuntimeError(f"{what} cannot be traced without the compiled binding")
+    if _tracing() and not (traced and ops() is not None):
+        raise RuntimeError(f"{what} cannot be traced{' without the compiled binding' if traced else ''}")

@@ -81,6 +81,8 @@ class CosAttnDecodeState:
             out = m.decode_steps(self.state, q, k, v, norm_const, self.cur_s)
             self.cur_s += T
             return out
+        # (a trace would hold the position of the call that it saw)
+        _binding.refuse_transforms("CosAttnDecodeState.step", self.state, q, k, v, norm_const, traced=False)
         if k.numel() != q.numel() or v.numel() != B * H * T * Dv or self.state.numel() < B * H * Dv * Dk:
             raise RuntimeError(f"q, k, v and the state do not fit each other: {list(q.shape)}, {list(k.shape)}, {list(v.shape)}, {list(self.state.shape)}")
         q, k, v = q.contiguous(), k.to(q.dtype).contiguous(), v.to(q.dtype).contiguous()
