@@ -129,3 +129,17 @@ def test_saved_tensor_hooks_and_modified_inputs():
         q.mul_(2)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.backward(do)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_compiled_functions_run_the_operators(name):
+    f, a = _functions()[name], _x(50, 2)[0]
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda t: f(t * 1) * 2, backend="aot_eager")
+    assert torch.equal(compiled(a), f(a) * 2)
+    if name not in ("prefill", "step"):
+        res = []
+        for call in (compiled, lambda t: f(t * 1) * 2):
+            leaf = a.clone().requires_grad_()
+            res.append(torch.autograd.grad(call(leaf).float().square().sum(), leaf)[0])
+        assert torch.equal(*res)
