@@ -691,6 +691,7 @@ struct Tables {
   cott_rotary_tables t = {};
   bool there = false;
   Tables(const OptTensor& s, const OptTensor& c, const at::Tensor& q) {
+    TORCH_CHECK(has(s) == has(c), "rotary takes the sines and the cosines, one of them is missing");
     if (!has(s)) return;
     auto dense = [&](const at::Tensor& x) { return dense16(x.scalar_type() == at::kFloat && x.device() == q.device() ? x : x.to(q.device(), at::kFloat)); };
     sin = dense(*s), cos = dense(*c);

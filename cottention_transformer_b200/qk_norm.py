@@ -32,6 +32,10 @@ def _check(q, k, q_weight, k_weight):
 def _tables(rotary, q):
     if rotary is None:
         return None, None
+    if (rotary[0] is None) != (rotary[1] is None):
+        raise RuntimeError("rotary takes the sines and the cosines, one of them is missing")
+    if rotary[0] is None:
+        return None, None
     sin, cos = (t.to(device=q.device, dtype=torch.float32).contiguous() for t in rotary)
     B, _, N, D = q.shape
     rot = 2 * sin.shape[-1]
