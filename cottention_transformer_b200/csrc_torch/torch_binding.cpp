@@ -676,12 +676,12 @@ at::Tensor gated_step(const at::Tensor& state, const at::Tensor& q_, const at::T
   const at::Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty_like(v);
+  state.unsafeGetTensorImpl()->bump_version();  // (refuses an inference tensor outside of inference mode: before it is written to)
   cott_gated_layout lay = {};
   lay.q = strides3(q), lay.k = strides3(k), lay.v = strides3(v), lay.out = strides3(out), lay.gate = strides3(log_decay);
   check(cott_gated_step(state.data_ptr<float>(), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), out.data_ptr(), &lay, (int)q.size(0),
                         (int)q.size(1), (int)q.size(2), (int)q.size(3), dtype_code(q.scalar_type()), dtype_code(log_decay.scalar_type()), stream_of(q)),
         "cott_gated_step");
-  state.unsafeGetTensorImpl()->bump_version();
   return out;
 }
 

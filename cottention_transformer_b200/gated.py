@@ -170,6 +170,8 @@ def gated_scan_step(state, q, k, v, log_decay):
     _check_state("state", state, q)
     if not state.is_contiguous() or state.data_ptr() % 16:
         raise RuntimeError("the state is updated in place: it must be contiguous and 16-byte aligned")
+    if state.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError("Inplace update to inference tensor outside InferenceMode is not allowed: the state was made in inference mode")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (state, q, k, v, log_decay)):
         raise RuntimeError("gated_scan_step is not differentiable: use gated_scan, or call it under torch.no_grad()")
     q, k, v = rows16(q), rows16(k), rows16(v)

@@ -115,3 +115,20 @@ def test_decays_inside_documents_of_a_few_tokens(dtype, D, N, roles, gate):
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 32), (torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 32), (torch.float16, 32)])
 def test_gradients_before_a_dropped_state_gradient_on_cuda_cores(dtype, D, at, held):
     _before_a_drop(dtype, D, at, held)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_a_state_of_inference_mode(compiled, monkeypatch):
+    """As torch's own in-place operators: written to inside inference mode, refused outside of it, before anything is written."""
+    from cottention_transformer_b200 import GatedScanState, _binding
+    if not compiled:
+        monkeypatch.setattr(_binding, "autograd", lambda: None)
+    x = [t.cuda() for t in _inputs(1, 2, 1, 64, torch.bfloat16, seed=44)[:4]]
+    with torch.inference_mode():
+        s = GatedScanState(1, 2, 64)
+        s.step(*x)
+        before = s.state.clone()
+    assert before.abs().sum() > 0
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        s.step(*x)
+    assert torch.equal(s.state, before)
