@@ -33,9 +33,8 @@ int check_state(const char* name, const void* p) {
   return reinterpret_cast<uintptr_t>(p) & 15 ? fail(COTT_ERR_ALIGN, "%s must be 16-byte aligned", name) : COTT_OK;
 }
 
-GatedArgs args_of(const cott_gated_layout* l, int B, int H, int N, int D, int gate_dtype) {
+GatedArgs args_of(const cott_gated_layout* l, int H, int N, int D, int gate_dtype) {
   GatedArgs g = {};
-  (void)B;
   const cott_strides d = dense(H, N, D), gd = {(long long)H * N, N, 1};
   g.sq = l ? l->q : d, g.sk = l ? l->k : d, g.sv = l ? l->v : d, g.so = l ? l->out : d;
   g.sdq = l ? l->dq : d, g.sdk = l ? l->dk : d, g.sdv = l ? l->dv : d;
@@ -75,20 +74,19 @@ int run_bwd(const GatedArgs& g, long states, cudaStream_t stream) {
   COTT_CUDA_TRY(launch_pdl(gated_dgate_kernel<T, D>, dim3((unsigned)(states * g.nchunks)), kGsThreads, 0, stream, g));
   return COTT_OK;
 }
-template <bool FWD, typename T>
-int run_dim(const GatedArgs& g, int D, long states, cudaStream_t stream) {
-  switch (D) {
-    case 32: return FWD ? run_fwd<T, 32>(g, states, stream) : run_bwd<T, 32>(g, states, stream);
-    case 64: return FWD ? run_fwd<T, 64>(g, states, stream) : run_bwd<T, 64>(g, states, stream);
-    default: return FWD ? run_fwd<T, 128>(g, states, stream) : run_bwd<T, 128>(g, states, stream);
-  }
+// float32 at every head dim; the 16-bit types at 32 (64 and 128 are the tensor cores')
+template <bool FWD, typename T, int D>
+int run_one(const GatedArgs& g, long states, cudaStream_t stream) {
+  return FWD ? run_fwd<T, D>(g, states, stream) : run_bwd<T, D>(g, states, stream);
 }
 template <bool FWD>
 int run_any(const GatedArgs& g, int D, int dtype, long states, cudaStream_t stream) {
-  switch (dtype) {
-    case COTT_F32: return run_dim<FWD, float>(g, D, states, stream);
-    case COTT_F16: return run_dim<FWD, __half>(g, D, states, stream);
-    default: return run_dim<FWD, __nv_bfloat16>(g, D, states, stream);
+  if (dtype == COTT_F16) return run_one<FWD, __half, 32>(g, states, stream);
+  if (dtype == COTT_BF16) return run_one<FWD, __nv_bfloat16, 32>(g, states, stream);
+  switch (D) {
+    case 32: return run_one<FWD, float, 32>(g, states, stream);
+    case 64: return run_one<FWD, float, 64>(g, states, stream);
+    default: return run_one<FWD, float, 128>(g, states, stream);
   }
 }
 
@@ -137,7 +135,7 @@ int cott_gated_scan_fwd(const void* q, const void* k, const void* v, const void*
       COTT_CUDA_TRY(cudaMemcpyAsync(final_state, initial_state, bytes, cudaMemcpyDeviceToDevice, s));
     return COTT_OK;
   }
-  GatedArgs g = args_of(layout, B, H, N, D, gate_dtype);
+  GatedArgs g = args_of(layout, H, N, D, gate_dtype);
   if ((st = check_rows("q", q, g.sq, dtype)) || (st = check_rows("k", k, g.sk, dtype)) || (st = check_rows("v", v, g.sv, dtype)) ||
       (st = check_rows("out", out, g.so, dtype)))
     return st;
@@ -177,7 +175,7 @@ int cott_gated_scan_bwd(const void* q, const void* k, const void* v, const void*
       COTT_CUDA_TRY(cudaMemcpyAsync(dinitial_state, dfinal_state, bytes, cudaMemcpyDeviceToDevice, s));
     return COTT_OK;
   }
-  GatedArgs g = args_of(layout, B, H, N, D, gate_dtype);
+  GatedArgs g = args_of(layout, H, N, D, gate_dtype);
   if ((st = check_rows("q", q, g.sq, dtype)) || (st = check_rows("k", k, g.sk, dtype)) || (st = check_rows("v", v, g.sv, dtype)) ||
       (st = check_rows("dout", dout, g.so, dtype)) || (st = check_rows("dq", dq, g.sdq, dtype)) || (st = check_rows("dk", dk, g.sdk, dtype)) ||
       (st = check_rows("dv", dv, g.sdv, dtype)))
@@ -200,7 +198,7 @@ int cott_gated_step(float* state, const void* q, const void* k, const void* v, c
   int st = check_sizes("cott_gated_step", B, H, T, D, dtype, gate_dtype);
   if (st) return st;
   if ((long)B * H * T == 0) return COTT_OK;
-  const GatedArgs g = args_of(layout, B, H, T, D, gate_dtype);
+  const GatedArgs g = args_of(layout, H, T, D, gate_dtype);
   if ((st = check_rows("q", q, g.sq, dtype)) || (st = check_rows("k", k, g.sk, dtype)) || (st = check_rows("v", v, g.sv, dtype)) ||
       (st = check_rows("out", out, g.so, dtype)))
     return st;
