@@ -1191,6 +1191,30 @@ int cott_selftest_device_wait(int polls, int code, int chunk, void* stream) {
   return COTT_OK;
 }
 
+static const char* wait_name(int code) {  // what the kWait* codes of the kernels stand for
+  switch (code) {
+    case 1: return "TMA";
+    case 2: return "free stage";
+    case 3: return "scores";
+    case 4: return "scores read";
+    case 5: return "prepared operand";
+    case 6: return "accumulator";
+    case 7: return "free accumulator";
+    case 8: return "state";
+    case 9: return "output";
+    case 10: return "gradient of the state";
+    case 11: return "staging buffer";
+    case 14: return "alignment of shared memory";
+    case 16: return "gated walk: TMA";
+    case 17: return "gated scan: free stage";
+    case 18: return "gated walk: weighted operand";
+    case 19: return "gated walk: state update";
+    case 20: return "gated chunk: TMA";
+    case 21: return "gated chunk: MMA";
+    default: return "unknown";
+  }
+}
+
 int cott_check_status(int* detail) {
   int v = 0;
   COTT_CUDA_TRY(cudaDeviceSynchronize());
@@ -1205,8 +1229,7 @@ int cott_check_status(int* detail) {
   if (v == 0) v = of_gated;
   if (detail) *detail = v;
   if (v != 0) {
-    return fail(COTT_ERR_DEVICE_WAIT, "a device-side wait gave up: stage %d (1=TMA, 2=score MMA, 3=accumulator MMA) at chunk %d",
-                v >> 16, v & 0xffff);
+    return fail(COTT_ERR_DEVICE_WAIT, "a device-side wait gave up: stage %d (%s) at chunk %d", v >> 16, wait_name(v >> 16), v & 0xffff);
   }
   return COTT_OK;
 }

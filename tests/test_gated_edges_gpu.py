@@ -132,3 +132,13 @@ def test_a_state_of_inference_mode(compiled, monkeypatch):
     with pytest.raises(RuntimeError, match="[Ii]nference"):
         s.step(*x)
     assert torch.equal(s.state, before)
+
+
+@pytest.mark.parametrize("code,name", [(1, "TMA"), (6, "accumulator"), (19, "gated walk: state update"), (21, "gated chunk: MMA")])
+def test_a_wait_that_gave_up_is_named(code, name):
+    """(The self-test's kernel polls a barrier four times, records the code and ends.)"""
+    from cottention_transformer_b200 import _lib
+    _lib.check(_lib.lib().cott_selftest_device_wait(4, code, 5, _lib.stream_ptr(torch.device("cuda"))), "selftest")
+    with pytest.raises(RuntimeError, match=rf"stage {code} \({name}\) at chunk 5"):
+        _lib.check_device_status()
+    _lib.check_device_status()
