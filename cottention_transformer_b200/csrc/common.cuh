@@ -114,6 +114,22 @@ cudaError_t launch_pdl(K kernel, dim3 grid, unsigned threads, size_t smem, cudaS
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Two products, two multiply-adds in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 // One pair of the rotary embedding ("rotate every two"): (x, y) -> (x c - y s, y c + x s).  Spelled with explicit
 // roundings so that every kernel that rotates -- the stand-alone pass and the causal kernels that rotate their tiles
 // in shared memory -- produces the same bits.

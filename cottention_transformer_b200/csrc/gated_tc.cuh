@@ -574,21 +574,6 @@ __device__ __forceinline__ void row_drops(const DropBits& drops, int wq, int lan
   seen = seen_bits<LOWER>(d, lane);
   if (d & (LOWER ? here : ~here)) block = 0.f;
 }
-// Two products, two multiply-adds in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 c;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
-      : "=f"(c.x), "=f"(c.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return c;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
 __device__ __forceinline__ float2 pair(const uint32_t* r) { return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
 // acc += 16 values times two packed pieces of a row
 template <typename T>

@@ -7,6 +7,7 @@
 // HBM-bound: every input is read once and every output written once; the backward recomputes r from x.  The gradient of a weight is
 // summed in registers over the rows of a thread, over the CTA in shared memory and over the CTAs by a second small kernel, all in a
 // fixed order.
+// (Packed arithmetic, mul2 and fma2: the pass is as much bound by its instructions as by memory.)
 #include "common.cuh"
 
 using namespace cott;
@@ -83,21 +84,6 @@ __device__ __forceinline__ float row_sum(float x) {
 #pragma unroll
   for (int off = LPR / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
   return x;
-}
-// Two products, two multiply-adds in one instruction (the pass is as much bound by its instructions as by memory).
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 c;
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}"
-      : "=f"(c.x), "=f"(c.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return c;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // the lane's E weights
