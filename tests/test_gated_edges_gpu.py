@@ -142,3 +142,54 @@ def test_a_wait_that_gave_up_is_named(code, name):
     with pytest.raises(RuntimeError, match=rf"stage {code} \({name}\) at chunk 5"):
         _lib.check_device_status()
     _lib.check_device_status()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_generation(dtype, D):
+    """A prompt with a mask and a token loop (norm with rotation, step) in two graphs that share a memory pool and a state, replayed in
+    turn with new inputs."""
+    from cottention_transformer_b200 import GatedScanState, qk_norm_rotary
+    B, H, N = 2, 3, 200
+    runs = [[t if t is None else t.cuda() for t in _inputs(B, H, N + 1, D, dtype, seed=s, masked=True)] for s in (45, 46)]
+    w = torch.rand(2, D, device="cuda") + 0.5
+    ang = torch.rand(1, 8, device="cuda")
+
+    def prompt(state, q, k, v, g, keep):
+        state.reset()
+        return state.prefill(*qk_norm_rotary(q, k, w[0], w[1]), v, g, keep=keep)
+
+    def token(state, q, k, v, g):
+        return state.step(*qk_norm_rotary(q, k, w[0], w[1], rotary=(ang.sin(), ang.cos())), v, g)
+
+    def split(x):
+        q, k, v, g, keep = x[:5]
+        return [t[:, :, :N].clone() for t in (q, k, v, g)] + [keep[:, :N].clone()], [t[:, :, N:].clone() for t in (q, k, v, g)]
+
+    want = []
+    with torch.no_grad():
+        for x in runs:
+            state, (a, b) = GatedScanState(B, H, D), split(x)
+            want.append([t.clone() for t in (prompt(state, *a), token(state, *b), token(state, *b), state.state)])
+        state, (a, b) = GatedScanState(B, H, D), split(runs[0])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            prompt(state, *a)
+            token(state, *b)
+        torch.cuda.synchronize()
+        first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first):
+            out_a = prompt(state, *a)
+        with torch.cuda.graph(second, pool=first.pool()):
+            out_b = token(state, *b)
+        for i in (1, 0, 1):
+            new_a, new_b = split(runs[i])
+            for s, t in zip(a + b, new_a + new_b):
+                s.copy_(t)
+            first.replay()
+            got = [out_a.clone()]
+            for _ in range(2):
+                second.replay()
+                got.append(out_b.clone())
+            assert all(torch.equal(s, t) for s, t in zip((*got, state.state), want[i]))
