@@ -4,11 +4,19 @@
 //   gated_walk_kernel   walks a sequence (or a segment of it) with the fp32 state in registers, S <- A S + K^T diag(e^(G_last-G_s)) V
 //                       (backwards: R <- A R + Q^T diag(e^(G_t)) dO), and leaves the state before (after) every chunk in memory as
 //                       the 16-bit operand that the other kernel wants.  The weighted operand is split into a 16-bit head and a
-//                       16-bit tail, two MMAs, so that a state is exact to about 2^-17: it lasts for the rest of the sequence.
+//                       16-bit tail, two MMAs, so that the fp32 state is exact to about 2^-17: it lasts for the rest of the sequence.
 //   gated_fwd_tc_kernel, gated_bwd64_kernel, gated_bwd128_kernel   take the chunks, none of which waits for another: scores by MMA,
 //                       decayed, masked and rounded to 16 bits in registers, back to TMEM as the A operand of the product with the rows; the state's part in
 //                       fp32, scaled by the row factor, beside it.
-// HBM-bound: the walk reads two tensors and writes half of one, the chunks read three and half of one, backwards four and a whole.
+// Traffic, in tensors (a chunk's state is half a tile at head dim 64, a whole one at 128): the walk reads two and writes the states; the
+// chunks read three and the states and write one, backwards four and both states and write three.  Walk and forward run at 0.64 - 0.84 of
+// the copy rate; the D 128 backward waits for the loads of its one chunk, the D 64 backward for the round trips of its groups (44 % of
+// the DRAM peak, no single part bounds it).
+//
+// Roundings to 16 bits beside those of the results, half a step each: the decayed scores, as the A operand of the product with the
+// rows; the copy of a state that multiplies rows, twice in a walk in segments (as the sum of its segment, and with the state before
+// that added).  <S, R> in the gradient of the gates is taken from those copies.  Together with the result's own rounding: 0.6 half steps
+// from 64 bits in the 2-norm (0.43 by the result's alone), the gates' gradient up to 0.8.
 //
 // The decays of a chunk: D_ts = e^(G_t - G_s) of the 32 x 32 blocks on the diagonal are taken element by element; a block below it
 // is the product of a row factor e^(G_t - G_b) and a column factor e^(G_b - G_s) with b the last position before the block's
@@ -1194,9 +1202,9 @@ __global__ void __launch_bounds__(kBwd128Threads, 1) gated_bwd128_kernel(const _
 //   last rows of this one are written, and no working warp spends its time on issuing
 // Two stages of (dO, V, K, Q, S, R), 80 KB, and a tile per group for its results, so that a stage is free as soon as the last group
 // has its products (staged over the tiles instead, a stage was held until the stores had been read: 2000 of a chunk's 8000 cycles).
-// B8 H16 N4096 bf16: 137 us, 3.6 TB/s; its traffic, states included, would take 83.  No single part bounds it (of 139 in one run:
-// 129 without the decays, 136 without the dot products, 135 without writing dg); the schedulers issue in 64 % of the cycles, and each group
-// waits for its own MMAs.  (One accumulator of 64 columns per group, half as many MMAs, is no faster: 136, and 1 % more for a
+// B8 H16 N4096 bf16: 144 us, 3.4 TB/s; its traffic, states included, would take 83.  No single part bounds it (of 139 in one run of an
+// earlier form: 129 without the decays, 136 without the dot products, 135 without writing dg; what keeps a dropped state and masked rows
+// out takes 7 of the 144); the schedulers issue in 64 % of the cycles, and each group waits for its own MMAs.  (One accumulator of 64 columns per group, half as many MMAs, is no faster: 136, and 1 % more for a
 // forward and a backward in turn.  L2 prefetches of the chunk after the next cost 8.)
 // 128 TMEM columns per group, of which half h has 64: scores, then 32 of packed scores and 32 of the accumulator; 64 each for the
 // state's part of dq and dk.

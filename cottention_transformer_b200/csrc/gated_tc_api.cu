@@ -9,8 +9,9 @@ constexpr int kSms = 148;  // (sizes of buffers follow from it: a constant, so t
 
 int tc_chunks(int N) { return (N + kGtChunk - 1) / kGtChunk; }
 
-// Into how many segments the walk of a sequence is cut: as many as there are SMs to spare, where that saves more than the two short
-// kernels behind it cost (a chunk of a walk takes about 1 us, they take about 10).
+// Into how many segments the walk of a sequence is cut: as many as fit beside each other on the SMs, where that saves more than the two
+// short kernels behind it cost (a chunk of a walk takes about 1 us, they take about 10).  (A walk's CTA fills an SM.  From 75 walks on,
+// one each, SMs stay idle, and from 149 on a second wave follows: cutting those walks too is not done.)
 int walk_segments(long walks, int n) {
   const int room = (int)(kSms / walks);
   if (room < 2) return 1;

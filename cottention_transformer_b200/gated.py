@@ -141,10 +141,15 @@ def gated_scan(q, k, v, log_decay, keep=None, initial_state=None, return_state=F
     initial_state: optional float32 ``[B, H, D, D]``, value index first.  Returns ``out``, in the memory order of ``v``, or
     ``(out, state)`` with ``return_state``: the state after the last position, in fp32.
 
-    Differentiable once in q, k, v, log_decay and initial_state (``return_state`` included).  A gate of ``-inf`` and the first gate of
-    a sequence without an initial state have no gradient.  16-bit tensors: the gradient of log_decay carries the roundings of the
-    16-bit products, also where log_decay is float32.  float16: a state entry beyond 65504 overflows, and what is smaller than the
-    type's smallest step (weights of less than 2^-24 within 128 positions) is lost."""
+    Differentiable once in q, k, v, log_decay and initial_state (``return_state`` included).  A gate of ``-inf`` (or below about -88,
+    where its decay is zero in float32) and the first gate of a sequence without an initial state have no gradient.
+
+    16-bit tensors at head dims 64 and 128: beside its own rounding a result carries those of the decayed scores and of the state's
+    copy that multiplies rows (0.6 half steps of the type in the 2-norm, 0.43 by the own rounding alone); the gradient of log_decay up
+    to 0.8, also where log_decay is float32.  The states themselves are fp32.  An infinity or NaN in an unmasked row reaches other
+    rows of its 128 positions, also those that do not see it.  float16: a state entry, or a score (``q.k``, in the backward
+    ``dout.v``) times its decay, beyond 65504 overflows, and what is smaller than the type's smallest step (weights of less than 2^-24
+    within 128 positions) is lost."""
     m = _binding.autograd()
     if m is not None:
         r = m.gated_scan(q, k, v, log_decay, keep, initial_state, bool(return_state))

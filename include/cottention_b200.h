@@ -428,7 +428,9 @@ int cott_cos_attn_bwd_rotary(const void* q, const void* k, const void* v, const 
  * the direction, 16-byte aligned, may be NULL where that is 0; its contents mean nothing between calls.
  * Rows are read and written 16 bytes at a time: base pointers and strides in multiples of 16 bytes (log_decay: any).
  * Sums and states are fp32.  At head dims 64 and 128 the 16-bit types run on the tensor cores: the decayed scores of a
- * chunk and the copy of a state that multiplies rows are rounded to the 16-bit type.  fp32 is fp32 throughout.
+ * chunk and the copy of a state that multiplies rows are rounded to the 16-bit type (few, long sequences: the copy twice),
+ * and in float16 overflow beyond 65504; a value that is not finite in an unmasked row reaches other rows of its 128
+ * positions.  fp32 is fp32 throughout.
  * NULL layout: dense [B, H, N, D] and [B, H, N]. */
 typedef struct cott_strides {
   long long b, h, n; /* elements from one batch entry, head, position to the next; the innermost dimension is contiguous */
