@@ -461,7 +461,9 @@ __global__ void __launch_bounds__(256) gated_seg_kernel(const GatedTcArgs a) {
 }
 
 // The states inside a segment += the decayed state before it.  A CTA per chunk and panel; most of those of a head that forgets within
-// a segment have nothing to do.  grid = B*H * nchunks * D/64, block = 128.
+// a segment have nothing to do.  The sum is fp32; what it starts from is the operand that the walk has rounded, so that a state that the
+// segment's start reaches carries two roundings.  (One would take the walk's fp32 states through memory, twice the bytes each way.)
+// grid = B*H * nchunks * D/64, block = 128.
 template <typename T, int D, bool REV>
 __global__ void __launch_bounds__(128) gated_patch_kernel(const GatedTcArgs a) {
   constexpr int NT = D / 64;
